@@ -15,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -23,6 +24,7 @@ CSRC_DIR = PKG_DIR / "csrc"
 INCLUDE_DIR = REPO_DIR / "include"
 LIB_NAME = "libagentkv_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+OBJ_DIR = PKG_DIR / "build"  # compiled sources, each rebuilt when it or a header is newer
 HOST_EXT_SRC = CSRC_DIR / "akv_pyhost.c"
 HOST_EXT_PATH = PKG_DIR / ("_akv_pyhost" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
@@ -84,13 +86,29 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not _stale():
         return LIB_PATH
     tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [_nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE_DIR}", "-shared", "-o", str(tmp)]
-    cmd += [str(p) for p in sources()]
-    if verbose:
-        print(" ".join(cmd))
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    flags = [*ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE_DIR}"]
+    headers = [*CSRC_DIR.glob("*.cuh"), *INCLUDE_DIR.glob("*.h")]
+    newest = max(p.stat().st_mtime for p in headers)
+    OBJ_DIR.mkdir(exist_ok=True)
+
+    def run(cmd: list[str]) -> None:
+        if verbose:
+            print(" ".join(cmd))
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+
+    def compile_one(src: Path) -> str:
+        obj = OBJ_DIR / (src.stem + ".o")
+        if force or not obj.exists() or obj.stat().st_mtime < max(newest, src.stat().st_mtime):
+            part = obj.with_suffix(".o.tmp")
+            run([_nvcc(), *flags, "-c", str(src), "-o", str(part)])
+            os.replace(part, obj)
+        return str(obj)
+
+    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:  # one nvcc per source
+        objs = list(pool.map(compile_one, sources()))
+    run([_nvcc(), *flags, "-shared", "-o", str(tmp), *objs])
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

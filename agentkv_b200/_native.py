@@ -42,6 +42,9 @@ ERROR_NAMES = {
     AKV_ERR_MIRROR: "replayed per-call log disagrees with the device state",
 }
 
+# ── element types (AKV_F32 ...) ───────────────────────────────────────────────
+F32, F16, BF16 = range(3)
+
 # ── ctl word indices ─────────────────────────────────────────────────────────
 CTL_FREE_LEFT = 0
 CTL_FREE_SIZE = 1
@@ -133,6 +136,38 @@ class AkvTreeView(C.Structure):
     ]
 
 
+class AkvPagedPool(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("total_blocks", C.c_int32),
+        ("num_layers", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("block_size", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("dtype", C.c_int32),
+        ("layer", C.c_int32),
+        ("_pad", C.c_int32),
+    ]
+
+
+class AkvPageBatch(C.Structure):
+    _fields_ = [
+        ("tables", C.c_void_p),
+        ("lengths", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("table_width", C.c_int32),
+        ("rows", C.c_int32),
+    ]
+
+
+class AkvHeads(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("stride_token", C.c_int64),
+        ("stride_head", C.c_int64),
+    ]
+
+
 _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
@@ -212,6 +247,18 @@ SIGNATURES = {
         [C.POINTER(AkvTreeView), _P, _P, _I32, _I64, _I32, _P, _P, _P, _P, _I32, _P, _I64, _P, _P],
     ),
 }
+
+_POOL, _BATCH, _HEADS = C.POINTER(AkvPagedPool), C.POINTER(AkvPageBatch), C.POINTER(AkvHeads)
+SIGNATURES.update({
+    "akv_kv_append": (C.c_int, [_POOL, _BATCH, _HEADS, _HEADS, _I32, _P, _P, _I32, _I32, _I32, _HEADS, _HEADS, _I32, _P,
+                                _P, _P]),
+    "akv_key_bounds": (C.c_int, [_POOL, _BATCH, _P, _P, _P]),
+    "akv_paged_attention_scratch_bytes": (C.c_int64, [_POOL, _I32, _I32, _I32, _I32]),
+    "akv_paged_attention": (C.c_int, [_POOL, _BATCH, _HEADS, _I32, C.c_float, _I32, _P, _I32, _HEADS, _P, _P, _I64, _P,
+                                      _P]),
+    "akv_select_blocks_scratch_bytes": (C.c_int64, [_I32, _I32, _I32, _I32]),
+    "akv_select_blocks": (C.c_int, [_POOL, _P, _BATCH, _HEADS, _I32, _I32, _I32, _I32, _P, _P, _I64, _P, _P]),
+})
 
 
 class NativeError(RuntimeError):

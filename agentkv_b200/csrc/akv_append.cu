@@ -1,0 +1,430 @@
+// akv_append.cu — new tokens' keys and values into the paged pool, rotated on
+// the way, and the bounds of the blocks that get them.
+//
+// Rotation: pair (x, y) of a token at position p becomes
+// (x cos a - y sin a, y cos a + x sin a), a = p * frequency of the pair; the
+// cosines and sines come from a table made once in 64 bits (an angle at
+// position 10^5 has lost 5 digits in 32 bits).  Products and sums in 32 bits,
+// rounded once to the pool's type.
+//
+// What bounds it: bytes moved (each operand row read and written once), and
+// for a decode step's few rows the launch and two dependent loads.
+//
+// Work: one unit per (row, block) that gets tokens, dealt to one or several
+// CTAs by heads; a thread takes one word (of kV elements, and the word of
+// their partners) of a head through the unit's tokens, so that a key's
+// bounds are that thread's own minimum and maximum: no atomics, and
+// the same result in any order.
+#include <climits>
+
+#include "akv_paged.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct AppendParams {
+  AkvLayer kv;
+  AkvTables tab;
+  const int32_t* starts;
+  int32_t n_tokens;
+  const char *key, *value, *query;
+  char* query_out;
+  int64_t k_tok, k_head, v_tok, v_head, q_tok, q_head, o_tok, o_head;  // strides in bytes
+  int32_t q_heads;
+  const float* rope;
+  int32_t rope_rows, rotary, interleaved;
+  char* bounds;
+  int64_t bounds_page, bounds_layer;  // bytes
+  AkvStatus* st;
+};
+
+// min / max that a NaN on either side makes NaN
+AKV_DEV float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+AKV_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// New tokens of row s, and how many blocks they fall into.
+AKV_DEV int32_t new_tokens(const AppendParams& p, int32_t s) {
+  if (p.starts == nullptr) return p.tab.lengths[s] > 0 ? 1 : 0;
+  const int32_t from = p.starts[s], to = p.starts[s + 1];
+  return from >= 0 && to <= p.n_tokens && to > from ? to - from : 0;
+}
+
+AKV_DEV int64_t blocks_touched(const AppendParams& p, int32_t s) {
+  const int32_t n = new_tokens(p, s), len = p.tab.lengths[s];
+  if (n == 0 || len < n) return 0;
+  const int bl = p.kv.bs_log2;
+  return ((len - 1) >> bl) - ((len - n) >> bl) + 1;
+}
+
+// Whether a pair's two elements lie in different words.
+AKV_DEV bool partners(const AppendParams& p, int elements) { return p.rope && (!p.interleaved || elements == 1); }
+
+// One word of a head: dimensions a .. a + kV - 1 and, where they are rotated
+// with other words, those of b.
+template <typename T, int kV>
+struct Lane {
+  int a, b;   // b < 0: one word only
+  int pair;   // first pair of the word in the table, -1: not rotated
+
+  AKV_DEV void set(const AppendParams& p, int w) {
+    const int half = p.rotary / 2;
+    const bool apart = partners(p, kV);
+    if (apart && w < half / kV) {
+      a = p.interleaved ? 2 * w : w * kV;
+      b = p.interleaved ? a + 1 : a + half;
+      pair = w * kV;
+      return;
+    }
+    if (apart) w += half / kV;  // behind the pairs' two words
+    a = w * kV;
+    b = -1;
+    pair = p.rope && a < p.rotary ? a / 2 : -1;
+  }
+};
+
+template <typename T, int kV>
+AKV_DEV void load_word(float (&x)[kV], const char* row, int d) {
+  const AkvVec<T, kV> w = *reinterpret_cast<const AkvVec<T, kV>*>(row + d * sizeof(T));
+#pragma unroll
+  for (int i = 0; i < kV; ++i) x[i] = to_f32<T>(w.v[i]);
+}
+
+// Rounds x to T (x holds the rounded values afterwards) and stores it.
+template <typename T, int kV>
+AKV_DEV void store_word(float (&x)[kV], char* row, int d) {
+  AkvVec<T, kV> w;
+#pragma unroll
+  for (int i = 0; i < kV; ++i) {
+    w.v[i] = from_f32<T>(x[i]);
+    x[i] = to_f32<T>(w.v[i]);
+  }
+  *reinterpret_cast<AkvVec<T, kV>*>(row + d * sizeof(T)) = w;
+}
+
+// x, y: the word(s) of one token at `pos`.
+template <typename T, int kV>
+AKV_DEV void rotate(const AppendParams& p, const Lane<T, kV>& ln, int32_t pos, float (&x)[kV], float (&y)[kV]) {
+  if (ln.pair < 0) return;
+  const float* cos_row = p.rope + static_cast<int64_t>(pos) * p.rotary;
+  const float* sin_row = cos_row + p.rotary / 2;
+  if (ln.b >= 0) {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+      const float c = cos_row[ln.pair + i], s = sin_row[ln.pair + i];
+      const float u = x[i], v = y[i];
+      x[i] = u * c - v * s;
+      y[i] = v * c + u * s;
+    }
+  } else if (kV > 1) {  // interleaved: kV / 2 whole pairs
+#pragma unroll
+    for (int i = 0; i < kV / 2; ++i) {
+      const float c = cos_row[ln.pair + i], s = sin_row[ln.pair + i];
+      const float u = x[2 * i], v = x[(2 * i + 1) % kV];
+      x[2 * i] = u * c - v * s;
+      x[(2 * i + 1) % kV] = v * c + u * s;
+    }
+  }
+}
+
+template <typename T, int kV>
+__global__ void __launch_bounds__(kThreads) k_append(AppendParams p) {
+  using Search = AkvRowSearch<kThreads>;
+  __shared__ typename Search::Shared sh;
+  if (akv_failed(p.st)) return;
+  const int bl = p.kv.bs_log2;
+  int32_t s;
+  int64_t rest = 0;
+  if (p.starts == nullptr) {
+    s = blockIdx.x;
+    if (threadIdx.x == 0 && blockIdx.y == 0 && p.tab.lengths[s] < 0)
+      akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, p.tab.lengths[s], 1);
+    if (new_tokens(p, s) == 0) return;
+  } else {
+    if (blockIdx.y == 0)
+      for (int32_t r = blockIdx.x * kThreads + threadIdx.x; r < p.tab.rows; r += gridDim.x * kThreads) {
+        const int32_t from = p.starts[r], to = p.starts[r + 1];
+        if (from < 0 || to < from || to > p.n_tokens || p.tab.lengths[r] < to - from)
+          akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, r, p.tab.lengths[r], to - from);
+      }
+    auto units = [&](int32_t r) { return blocks_touched(p, r); };
+    Search search;
+    search.scan(sh, p.tab.rows, units);
+    if (blockIdx.x >= search.total) return;
+    search.find(sh, blockIdx.x, units, s, rest);
+  }
+  const int32_t len = p.tab.lengths[s], n = new_tokens(p, s), old = len - n;
+  const int32_t block = (old >> bl) + static_cast<int32_t>(rest);
+  const int64_t from = static_cast<int64_t>(block) << bl, to = from + (1 << bl);
+  const int32_t p0 = old > from ? old : static_cast<int32_t>(from);
+  const int32_t p1 = len < to ? len : static_cast<int32_t>(to);
+  // the first token's row in the operands
+  const int64_t row0 = (p.starts ? p.starts[s] : s) + static_cast<int64_t>(p0 - old);
+  const int32_t id = block < p.tab.width ? p.tab.ids[s * p.tab.stride + block] : -1;
+  const bool placed = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.kv.total);
+  const bool turned = p.rope == nullptr || p1 <= p.rope_rows;
+  if (!placed || !turned) {
+    if (threadIdx.x == 0 && blockIdx.y == 0)
+      akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, placed ? p1 - 1 : id, placed ? p.rope_rows : p.kv.total);
+    return;
+  }
+  const int32_t in0 = static_cast<int32_t>(p0 - from), count = p1 - p0;
+  char* page = p.kv.base + id * p.kv.page_bytes;
+  // words of a head: a rotated one with its partner counts once
+  const int all = p.kv.dim / kV;
+  const int words = partners(p, kV) ? all - p.rotary / 2 / kV : all;
+  const int32_t heads = p.kv.heads;
+  const int64_t items = static_cast<int64_t>(heads) * (words + all) + static_cast<int64_t>(p.q_heads) * words;
+  for (int64_t it = blockIdx.y * kThreads + threadIdx.x; it < items; it += static_cast<int64_t>(gridDim.y) * kThreads) {
+    if (it < static_cast<int64_t>(heads) * words) {  // a key
+      const int32_t h = static_cast<int32_t>(it / words);
+      Lane<T, kV> ln;
+      ln.set(p, static_cast<int>(it % words));
+      char* tile = page + h * p.kv.tile_bytes;
+      float lo[kV], hi[kV], lo2[kV], hi2[kV];
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        lo[i] = lo2[i] = INFINITY;
+        hi[i] = hi2[i] = -INFINITY;
+      }
+      auto take = [&](const float(&x)[kV], const float(&y)[kV]) {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          lo[i] = min_nan(lo[i], x[i]);
+          hi[i] = max_nan(hi[i], x[i]);
+          lo2[i] = min_nan(lo2[i], y[i]);
+          hi2[i] = max_nan(hi2[i], y[i]);
+        }
+      };
+      if (p.bounds)
+#pragma unroll 4
+        for (int32_t r = 0; r < in0; ++r) {
+          float x[kV], y[kV] = {};
+          load_word<T, kV>(x, tile + r * p.kv.row_bytes, ln.a);
+          if (ln.b >= 0) load_word<T, kV>(y, tile + r * p.kv.row_bytes, ln.b);
+          take(x, y);
+        }
+#pragma unroll 4
+      for (int32_t t = 0; t < count; ++t) {
+        const char* src = p.key + (row0 + t) * p.k_tok + h * p.k_head;
+        char* dst = tile + static_cast<int64_t>(in0 + t) * p.kv.row_bytes;
+        float x[kV], y[kV] = {};
+        load_word<T, kV>(x, src, ln.a);
+        if (ln.b >= 0) load_word<T, kV>(y, src, ln.b);
+        rotate<T, kV>(p, ln, p0 + t, x, y);
+        store_word<T, kV>(x, dst, ln.a);
+        if (ln.b >= 0) store_word<T, kV>(y, dst, ln.b);
+        take(x, y);
+      }
+      if (p.bounds) {
+        char* b = p.bounds + id * p.bounds_page + p.bounds_layer + static_cast<int64_t>(h) * 2 * p.kv.row_bytes;
+        store_word<T, kV>(lo, b, ln.a);
+        store_word<T, kV>(hi, b + p.kv.row_bytes, ln.a);
+        if (ln.b >= 0) {
+          store_word<T, kV>(lo2, b, ln.b);
+          store_word<T, kV>(hi2, b + p.kv.row_bytes, ln.b);
+        }
+      }
+    } else if (it < static_cast<int64_t>(heads) * (words + all)) {  // a value: bits only
+      const int64_t i = it - static_cast<int64_t>(heads) * words;
+      const int32_t h = static_cast<int32_t>(i / all);
+      const int d = static_cast<int>(i % all) * kV * static_cast<int>(sizeof(T));
+      const char* src = p.value + row0 * p.v_tok + h * p.v_head + d;
+      char* dst = page + p.kv.kv_bytes + h * p.kv.tile_bytes + static_cast<int64_t>(in0) * p.kv.row_bytes + d;
+#pragma unroll 4
+      for (int32_t t = 0; t < count; ++t)
+        *reinterpret_cast<AkvVec<T, kV>*>(dst + static_cast<int64_t>(t) * p.kv.row_bytes) =
+            *reinterpret_cast<const AkvVec<T, kV>*>(src + t * p.v_tok);
+    } else {  // a query
+      const int64_t i = it - static_cast<int64_t>(heads) * (words + all);
+      const int32_t h = static_cast<int32_t>(i / words);
+      Lane<T, kV> ln;
+      ln.set(p, static_cast<int>(i % words));
+#pragma unroll 4
+      for (int32_t t = 0; t < count; ++t) {
+        const char* src = p.query + (row0 + t) * p.q_tok + h * p.q_head;
+        char* dst = p.query_out + (row0 + t) * p.o_tok + h * p.o_head;
+        float x[kV], y[kV] = {};
+        load_word<T, kV>(x, src, ln.a);
+        if (ln.b >= 0) load_word<T, kV>(y, src, ln.b);
+        rotate<T, kV>(p, ln, p0 + t, x, y);
+        store_word<T, kV>(x, dst, ln.a);
+        if (ln.b >= 0) store_word<T, kV>(y, dst, ln.b);
+      }
+    }
+  }
+}
+
+// The bounds of every block of every row, from its keys: one warp per (row,
+// block, head), a lane per element.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_bounds(AppendParams p) {
+  if (akv_failed(p.st)) return;
+  const int lane = threadIdx.x & 31, bl = p.kv.bs_log2;
+  const int64_t per_row = static_cast<int64_t>(p.tab.width) * p.kv.heads;
+  const int64_t items = p.tab.rows * per_row;
+  for (int64_t it = blockIdx.x * (kThreads / 32ll) + threadIdx.x / 32; it < items; it += gridDim.x * (kThreads / 32ll)) {
+    const int32_t s = static_cast<int32_t>(it / per_row);
+    const int32_t block = static_cast<int32_t>(it % per_row / p.kv.heads), h = static_cast<int32_t>(it % p.kv.heads);
+    const int32_t len = akv_held(p.tab, bl, s);
+    if (block == 0 && h == 0 && lane == 0 && p.tab.lengths[s] > len)
+      akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, p.tab.lengths[s], p.tab.width);
+    const int64_t from = static_cast<int64_t>(block) << bl;
+    if (from >= len) continue;
+    const int32_t rows = static_cast<int32_t>(len - from < (1 << bl) ? len - from : (1 << bl));
+    const int32_t id = p.tab.ids[s * p.tab.stride + block];
+    if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.kv.total)) {
+      if (h == 0 && lane == 0) akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, id, p.kv.total);
+      continue;
+    }
+    const char* tile = p.kv.base + id * p.kv.page_bytes + h * p.kv.tile_bytes;
+    char* b = p.bounds + id * p.bounds_page + p.bounds_layer + static_cast<int64_t>(h) * 2 * p.kv.row_bytes;
+    for (int d = lane; d < p.kv.dim; d += 32) {
+      float lo = INFINITY, hi = -INFINITY;
+#pragma unroll 8
+      for (int32_t r = 0; r < rows; ++r) {
+        const float x = to_f32<T>(reinterpret_cast<const T*>(tile + static_cast<int64_t>(r) * p.kv.row_bytes)[d]);
+        lo = min_nan(lo, x);
+        hi = max_nan(hi, x);
+      }
+      reinterpret_cast<T*>(b)[d] = from_f32<T>(lo);
+      reinterpret_cast<T*>(b + p.kv.row_bytes)[d] = from_f32<T>(hi);
+    }
+  }
+}
+
+using AppendKernel = void (*)(AppendParams);
+
+// `elements`: the largest word, in elements, that every address, stride and
+// the rotary half allow.
+template <typename T>
+AppendKernel append_kernel(int elements) {
+  if (elements >= 8 && sizeof(T) == 2) return k_append<T, 8>;
+  if (elements >= 4) return k_append<T, 4>;
+  if (elements >= 2) return k_append<T, 2>;
+  return k_append<T, 1>;
+}
+
+AppendKernel append_kernel(int32_t dtype, int elements) {
+  return dtype == AKV_F32 ? append_kernel<float>(elements)
+                          : dtype == AKV_F16 ? append_kernel<__half>(elements) : append_kernel<__nv_bfloat16>(elements);
+}
+
+AppendKernel bounds_kernel(int32_t dtype) {
+  return dtype == AKV_F32 ? k_bounds<float> : dtype == AKV_F16 ? k_bounds<__half> : k_bounds<__nv_bfloat16>;
+}
+
+int lowest_bit(uint64_t bits) { return static_cast<int>(bits & (~bits + 1) & 31); }
+
+}  // namespace
+
+int akv_append_prepare() {
+  for (int32_t dtype : {AKV_F32, AKV_F16, AKV_BF16}) {
+    for (int n : {1, 2, 4, 8})
+      if (int rc = akv_load_kernel(reinterpret_cast<const void*>(append_kernel(dtype, n)), "akv_prepare: k_append"))
+        return rc;
+    if (int rc = akv_load_kernel(reinterpret_cast<const void*>(bounds_kernel(dtype)), "akv_prepare: k_bounds"))
+      return rc;
+  }
+  return AKV_OK;
+}
+
+extern "C" int akv_kv_append(const AkvPagedPool* pool, const AkvPageBatch* batch, const AkvHeads* key,
+                             const AkvHeads* value, int32_t n_tokens, const int32_t* starts, const float* rope,
+                             int32_t rope_rows, int32_t rotary_dim, int32_t interleaved, const AkvHeads* query,
+                             const AkvHeads* query_out, int32_t n_query_heads, void* bounds, AkvStatus* status,
+                             void* stream) {
+  const char* what = "akv_kv_append";
+  AppendParams p = {};
+  if (int rc = akv_layer_view(what, pool, &p.kv)) return rc;
+  if (int rc = akv_tables_view(what, batch, pool->block_size, &p.tab)) return rc;
+  AKV_ARG_CHECK(n_tokens >= 0, "%s: n_tokens=%d", what, n_tokens);
+  AKV_ARG_CHECK(starts || n_tokens == p.tab.rows, "%s: %d tokens for %d rows of one token each", what, n_tokens,
+                p.tab.rows);
+  if (n_tokens == 0 || p.tab.rows == 0) return AKV_OK;
+  AKV_ARG_CHECK(pool->data && key && key->data && value && value->data, "%s: NULL pointer", what);
+  AKV_ARG_CHECK(n_query_heads >= 0 && (n_query_heads == 0 || (query && query->data && query_out && query_out->data)),
+                "%s: bad query", what);
+  AKV_ARG_CHECK(rope == nullptr || (rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= p.kv.dim && rope_rows >= 0),
+                "%s: rotary_dim=%d of head_dim %d, %d rows", what, rotary_dim, p.kv.dim, rope_rows);
+  const int es = akv_dtype_bytes(pool->dtype);
+  uint64_t bits = reinterpret_cast<uintptr_t>(pool->data) | static_cast<uint64_t>(p.kv.row_bytes) |
+                  reinterpret_cast<uintptr_t>(bounds);
+  for (const AkvHeads* x : {key, value, n_query_heads ? query : key, n_query_heads ? query_out : key}) {
+    AKV_ARG_CHECK(x->stride_token >= 0 && x->stride_head >= 0, "%s: negative stride", what);
+    AKV_ARG_CHECK(akv_aligned(x->data, es), "%s: misaligned pointer", what);
+    bits |= reinterpret_cast<uintptr_t>(x->data) | static_cast<uint64_t>(x->stride_token * es) |
+            static_cast<uint64_t>(x->stride_head * es);
+  }
+  AKV_ARG_CHECK(akv_aligned(rope, 4) && akv_aligned(bounds, es), "%s: misaligned pointer", what);
+  // a word lies wholly in one half of the rotated pairs, or holds whole pairs
+  if (rope) bits |= static_cast<uint64_t>(interleaved ? rotary_dim : rotary_dim / 2) * es;
+  const int low = lowest_bit(bits);
+  const int elements = (low == 0 || low > 16 ? 16 : low) / es;
+  p.starts = starts;
+  p.n_tokens = n_tokens;
+  p.key = static_cast<const char*>(key->data);
+  p.k_tok = key->stride_token * es;
+  p.k_head = key->stride_head * es;
+  p.value = static_cast<const char*>(value->data);
+  p.v_tok = value->stride_token * es;
+  p.v_head = value->stride_head * es;
+  p.q_heads = n_query_heads;
+  if (n_query_heads) {
+    p.query = static_cast<const char*>(query->data);
+    p.q_tok = query->stride_token * es;
+    p.q_head = query->stride_head * es;
+    p.query_out = static_cast<char*>(query_out->data);
+    p.o_tok = query_out->stride_token * es;
+    p.o_head = query_out->stride_head * es;
+  }
+  p.rope = rope;
+  p.rope_rows = rope_rows;
+  p.rotary = rope ? rotary_dim : 0;
+  p.interleaved = interleaved != 0;
+  p.bounds = static_cast<char*>(bounds);
+  p.bounds_layer = static_cast<int64_t>(p.kv.heads) * 2 * p.kv.row_bytes * pool->layer;
+  p.bounds_page = static_cast<int64_t>(p.kv.heads) * 2 * p.kv.row_bytes * pool->num_layers;
+  p.st = status;
+  // a row's n tokens lie in at most n, and at most n / block_size + 2, blocks
+  const int64_t most = n_tokens / pool->block_size + 2ll * p.tab.rows;
+  const int64_t units = starts == nullptr ? p.tab.rows : most < n_tokens ? most : n_tokens;
+  // as many CTAs per unit as its words fill, while there are SMs for them
+  const int64_t words = p.kv.dim / elements;
+  const int64_t items = words * (2ll * p.kv.heads + p.q_heads);
+  int64_t per = (items + kThreads - 1) / kThreads;
+  const int64_t room = (8ll * kAkvSMs + units - 1) / units;
+  per = per < room ? per : room;
+  const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(per < 1 ? 1 : per > 65535 ? 65535 : per));
+  append_kernel(pool->dtype, elements)<<<grid, kThreads, 0, akv_stream(stream)>>>(p);
+  AKV_LAUNCH_CHECK(what);
+  return AKV_OK;
+}
+
+extern "C" int akv_key_bounds(const AkvPagedPool* pool, const AkvPageBatch* batch, void* bounds, AkvStatus* status,
+                              void* stream) {
+  const char* what = "akv_key_bounds";
+  AppendParams p = {};
+  if (int rc = akv_layer_view(what, pool, &p.kv)) return rc;
+  if (int rc = akv_tables_view(what, batch, pool->block_size, &p.tab)) return rc;
+  if (p.tab.rows == 0 || p.tab.width == 0) return AKV_OK;
+  AKV_ARG_CHECK(pool->data && bounds, "%s: NULL pointer", what);
+  AKV_ARG_CHECK(akv_aligned(bounds, akv_dtype_bytes(pool->dtype)), "%s: misaligned pointer", what);
+  p.bounds = static_cast<char*>(bounds);
+  p.bounds_layer = static_cast<int64_t>(p.kv.heads) * 2 * p.kv.row_bytes * pool->layer;
+  p.bounds_page = static_cast<int64_t>(p.kv.heads) * 2 * p.kv.row_bytes * pool->num_layers;
+  p.st = status;
+  const int64_t warps = static_cast<int64_t>(p.tab.rows) * p.tab.width * p.kv.heads;
+  const int64_t ctas = (warps + kThreads / 32 - 1) / (kThreads / 32), most = 16ll * kAkvSMs;
+  bounds_kernel(pool->dtype)<<<static_cast<unsigned>(ctas < most ? ctas : most), kThreads, 0, akv_stream(stream)>>>(p);
+  AKV_LAUNCH_CHECK(what);
+  return AKV_OK;
+}

@@ -67,6 +67,9 @@ int akv_tree_prepare();
 int akv_fanout_prepare();
 int akv_kvio_prepare();
 int akv_agents_prepare();
+int akv_append_prepare();
+int akv_attend_prepare();
+int akv_select_prepare();
 
 #define AKV_ARG_CHECK(cond, ...)              \
   do {                                        \

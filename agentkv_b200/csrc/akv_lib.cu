@@ -118,5 +118,8 @@ extern "C" int akv_prepare(void) {
   if (int rc = akv_tree_prepare()) return rc;
   if (int rc = akv_kvio_prepare()) return rc;
   if (int rc = akv_agents_prepare()) return rc;
+  if (int rc = akv_append_prepare()) return rc;
+  if (int rc = akv_attend_prepare()) return rc;
+  if (int rc = akv_select_prepare()) return rc;
   return akv_fanout_prepare();
 }

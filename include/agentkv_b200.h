@@ -647,6 +647,122 @@ AKV_API int akv_mirror_take_log(AkvMirror* m, int32_t* dst, int64_t cap);
 AKV_API int akv_alloc_replay(const AkvAllocState* st, const int32_t* log, int64_t n_words, AkvStatus* status,
                              void* stream);
 
+/* ── attention over the paged pool ──────────────────────────────────────────
+ * What a model computes with the keys and values that the pool holds.  The
+ * reference assembles every sequence's K and V as contiguous tensors and
+ * leaves the attention to the model (agentkv/hf_cache.py:129-153); these
+ * entry points append to, rank and read the pages where they lie.
+ *
+ * AkvPagedPool names one layer of a contiguous pool
+ * [total_blocks][num_layers][2][num_kv_heads][block_size][head_dim];
+ * block_size is a power of two.  AkvPageBatch names a batch of `rows`
+ * sequences: row s holds lengths[s] tokens (0: a padding row), token t of it
+ * in block tables[s * table_stride + t / block_size], position
+ * t % block_size.  tables and lengths are DEVICE arrays; table entries behind
+ * a row's last block are not read.  Strides are in elements. */
+enum { AKV_F32 = 0, AKV_F16 = 1, AKV_BF16 = 2 };
+
+typedef struct AkvPagedPool {
+  void* data;
+  int32_t total_blocks;
+  int32_t num_layers;
+  int32_t num_kv_heads;
+  int32_t block_size;
+  int32_t head_dim;
+  int32_t dtype; /* AKV_F32 / AKV_F16 / AKV_BF16 */
+  int32_t layer;
+  int32_t _pad;
+} AkvPagedPool;
+
+typedef struct AkvPageBatch {
+  const int32_t* tables;
+  const int32_t* lengths;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t rows;
+} AkvPageBatch;
+
+/* A [tokens][heads][head_dim] operand: head_dim contiguous, strides in
+ * elements. */
+typedef struct AkvHeads {
+  void* data;
+  int64_t stride_token;
+  int64_t stride_head;
+} AkvHeads;
+
+/* New tokens' keys and values into the pages.  lengths counts the new tokens
+ * in: row s's starts[s + 1] - starts[s] new tokens are its last ones.  Their
+ * rows in key / value (and query) are starts[s] .. starts[s + 1] - 1; starts
+ * is a device array of rows + 1 ascending values in [0, n_tokens].  starts ==
+ * NULL: row s has one new token, row s of the operands (n_tokens == rows),
+ * and none where lengths[s] == 0.
+ *
+ * rope != NULL: the first rotary_dim dimensions of each new key (and of
+ * query's n_query_heads heads, written to query_out, which may be query) are
+ * rotated by the token's position in its sequence.  Row p of rope (float32
+ * [rope_rows][rotary_dim], 16-byte aligned) holds the cosines of position p's
+ * rotary_dim / 2 angles, then their sines.  Pair i is (i, i + rotary_dim / 2),
+ * or (2 i, 2 i + 1) with interleaved != 0.  Computed in 32 bits, rounded once.
+ *
+ * bounds != NULL: [total_blocks][num_layers][num_kv_heads][2][head_dim] of
+ * the pool's type, 16-byte aligned; of every block that gets a token, the
+ * minimum and maximum by dimension of all the keys that it then holds are
+ * written (made anew from the block's rows, so a copied block needs no copy of its
+ * bounds; NaN in a key makes both NaN).
+ *
+ * No two rows may append to the same block in one call.  A block id out of
+ * range, a position at or above rope_rows, or more new tokens than lengths
+ * says are reported (AKV_ERR_OUT_OF_RANGE) and those tokens skipped. */
+AKV_API int akv_kv_append(const AkvPagedPool* pool, const AkvPageBatch* batch, const AkvHeads* key,
+                  const AkvHeads* value, int32_t n_tokens, const int32_t* starts, const float* rope,
+                  int32_t rope_rows, int32_t rotary_dim, int32_t interleaved, const AkvHeads* query,
+                  const AkvHeads* query_out, int32_t n_query_heads, void* bounds, AkvStatus* status,
+                  void* stream);
+
+/* bounds (as above) of every block of every row, from the keys in the pool:
+ * for blocks that were written by other means than akv_kv_append. */
+AKV_API int akv_key_bounds(const AkvPagedPool* pool, const AkvPageBatch* batch, void* bounds, AkvStatus* status,
+                   void* stream);
+
+/* Attention of one new token of each row over the row's pages: query and out
+ * are [rows][num_kv_heads * group][head_dim] of the pool's type, query head i
+ * reads key head i / group.  Position t of row s takes part when
+ * t < lengths[s], and with window > 0 only when t >= lengths[s] - window.
+ * selected != NULL: int32 [rows][num_kv_heads][keep], places in the row's
+ * table (distinct, any order, the valid ones first and -1 behind them); only
+ * their positions take part.  Scores are scaled by `scale`; sums, the
+ * softmax's statistics and the output are held in 32 bits and the output is
+ * rounded once.  A row in which nothing takes part gives 0 (lse -inf).  lse, when
+ * non-NULL, is float32 [rows][num_kv_heads * group]: the natural logarithm
+ * of the sum of the scores' exponentials.
+ *
+ * scratch: akv_paged_attention_scratch_bytes() bytes of device memory, 16-byte
+ * aligned, for this call alone until it has run; no initial contents.  An
+ * id out of range is reported (AKV_ERR_OUT_OF_RANGE) and its positions left out. */
+AKV_API int64_t akv_paged_attention_scratch_bytes(const AkvPagedPool* pool, int32_t rows, int32_t table_width,
+                                          int32_t group, int32_t keep);
+AKV_API int akv_paged_attention(const AkvPagedPool* pool, const AkvPageBatch* batch, const AkvHeads* query,
+                        int32_t group, float scale, int32_t window, const int32_t* selected, int32_t keep,
+                        const AkvHeads* out, float* lse, void* scratch, int64_t scratch_bytes,
+                        AkvStatus* status, void* stream);
+
+/* The blocks of each row that matter most to its new token, by a bound on
+ * their keys' scores: for row s, key head h and block j of n =
+ * ceil(lengths[s] / block_size), with kmin, kmax the block's bounds (pool->data
+ * is not read, bounds is as for akv_kv_append),
+ *   score = sum over the group's query heads and d of max(q_d kmin_d, q_d kmax_d),
+ * in 64 bits.  selected [rows][num_kv_heads][keep] gets ascending places in
+ * the row's table, -1 behind them: all n where n <= keep; else the first
+ * `first` and the last `last` blocks (first + last <= keep) and the
+ * highest-scored of the others, the lowest place of equal ones.  A NaN score
+ * counts as the highest.  scratch: akv_select_blocks_scratch_bytes() bytes,
+ * 16-byte aligned, as above. */
+AKV_API int64_t akv_select_blocks_scratch_bytes(int32_t rows, int32_t num_kv_heads, int32_t table_width, int32_t keep);
+AKV_API int akv_select_blocks(const AkvPagedPool* pool, const void* bounds, const AkvPageBatch* batch,
+                      const AkvHeads* query, int32_t group, int32_t keep, int32_t first, int32_t last,
+                      int32_t* selected, void* scratch, int64_t scratch_bytes, AkvStatus* status,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif
