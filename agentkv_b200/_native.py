@@ -44,6 +44,7 @@ ERROR_NAMES = {
 
 # ── element types (AKV_F32 ...) ───────────────────────────────────────────────
 F32, F16, BF16 = range(3)
+ATTENTION_COUNTERS = 1536  # AKV_ATTENTION_COUNTERS
 
 # ── ctl word indices ─────────────────────────────────────────────────────────
 CTL_FREE_LEFT = 0
@@ -255,7 +256,7 @@ SIGNATURES.update({
     "akv_key_bounds": (C.c_int, [_POOL, _BATCH, _P, _P, _P]),
     "akv_paged_attention_scratch_bytes": (C.c_int64, [_POOL, _I32, _I32, _I32, _I32]),
     "akv_paged_attention": (C.c_int, [_POOL, _BATCH, _HEADS, _I32, C.c_float, _I32, _P, _I32, _HEADS, _P, _P, _I64, _P,
-                                      _P]),
+                                      _P, _P]),
     "akv_select_blocks_scratch_bytes": (C.c_int64, [_I32, _I32, _I32, _I32]),
     "akv_select_blocks": (C.c_int, [_POOL, _P, _BATCH, _HEADS, _I32, _I32, _I32, _I32, _P, _P, _I64, _P, _P]),
 })

@@ -42,6 +42,7 @@ from .kernels import _as_device_i32, _require_cuda, _status_buffer, raise_for_st
 
 _DTYPES = {torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
 _GRAPH_STATUS: dict = {}
+_COUNTERS: dict = {}
 _byref = ctypes.byref
 
 
@@ -58,6 +59,19 @@ def _status(device: torch.device, status: Optional[torch.Tensor]) -> Optional[to
     if device.index not in _GRAPH_STATUS:
         _GRAPH_STATUS[device.index] = torch.zeros(N.STATUS_BYTES // 4, dtype=torch.int32, device=device)
     return _status_buffer(device)
+
+
+def _counters(device: torch.device) -> torch.Tensor:
+    """The arrival counters of paged_attention, zero between calls: one
+    array per device and stream, and one of its own for a captured call, whose
+    replays may overlap other work of any stream."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(N.ATTENTION_COUNTERS, dtype=torch.int32, device=device)
+    key = (device.index, stream_handle(device))
+    buf = _COUNTERS.get(key)
+    if buf is None:
+        buf = _COUNTERS[key] = torch.zeros(N.ATTENTION_COUNTERS, dtype=torch.int32, device=device)
+    return buf
 
 
 def _pool_view(pool: torch.Tensor, layer: int, what: str) -> N.AkvPagedPool:
@@ -389,11 +403,12 @@ def paged_attention(query: torch.Tensor, pool: torch.Tensor, layer: int, tables,
     with _On(dev):
         st = _status(dev, status)
         scratch = _scratch(N.lib.akv_paged_attention_scratch_bytes(_byref(p), rows, b.table_width, group, keep), dev)
+        counters = _counters(dev)
         N.check(N.lib.akv_paged_attention(
             _byref(p), _byref(b), _byref(qview), group, dim ** -0.5 if scale is None else scale,
             min(window, (1 << 31) - 1), sel, keep, _byref(oview), None if lse is None else lse.data_ptr(),
             None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(),
-            None if st is None else st.data_ptr(), stream_handle(dev)))
+            counters.data_ptr(), None if st is None else st.data_ptr(), stream_handle(dev)))
         if check and st is not None:
             raise_for_status(st)
     return (out, lse) if return_lse else out

@@ -12,12 +12,14 @@
 // query heads that shares it (4 * group flops per 2-byte element pair), so the
 // time is the pool's bytes over the HBM rate.
 //
-// Work: (row, key head, up to kHeads query heads) pairs of chunks of 64
-// positions.  All chunks of the batch, in that order, are dealt to the CTAs in
-// equal contiguous ranges, whatever the rows' lengths are (the host does not know
-// them, and a captured launch replays with others): a pair that lies inside
-// one range is finished there, one that crosses ranges leaves a piece in
-// scratch per CTA, and k_join joins them.
+// Work: a pair is one row with one key head (or a part of its query heads,
+// where they are more than a product has columns), and its work is the row's
+// chunks of 64 positions.  All pairs' chunks, one behind another, are dealt to
+// the CTAs in equal contiguous ranges, whatever the rows' lengths are (the host
+// does not know them, and a captured launch replays with others).  A pair
+// inside one range is finished there; of one that crosses ranges each CTA
+// leaves a piece in scratch, and the last CTA to do so joins them (by 16s
+// where there are more).
 #include <climits>
 
 #include "akv_paged.cuh"
@@ -30,14 +32,14 @@ constexpr int kTile = 16;               // positions per warp and step
 constexpr int kChunk = kTile * kWarps;  // positions per CTA and step
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// Where nothing has been seen yet (a finite number: differences stay numbers).
+constexpr float kLowest = -3.402823466e38f;
 // A running maximum is raised only once a score lies this far above it (the
 // sums are the same for any m, so long as 2^(x - m) stays in range: at most
 // 2^8 here), which spares most steps the reduction over the lanes.
 constexpr float kLazy = 8.0f;
-
-struct AttendMeta {
-  int32_t row, head, part, pieces;
-};
+constexpr int kFan = 16;                   // pieces that are joined at a time
+constexpr int kMaxCtas = kFan * kFan * 2;  // two levels of joining
 
 struct AttendParams {
   AkvLayer kv;
@@ -52,13 +54,13 @@ struct AttendParams {
   int32_t group, parts;  // query heads per key head, and the pairs that they make
   float scale_log2;
   int32_t window;
-  int32_t direct;  // one CTA per pair, nothing to join
   float* pieces;
-  AttendMeta* meta;
+  int32_t* arrived;  // [3 * gridDim.x], zero between launches
   AkvStatus* st;
 };
 
-// Row s: positions [lo, n) take part; its pairs have chunks [first, first + chunks).
+// Row s: positions [lo, n) take part, in chunks [first, first + chunks) of the
+// row (of its selected blocks, where there is a selection).
 struct Extent {
   int32_t n, lo, first, chunks;
 };
@@ -68,71 +70,98 @@ AKV_DEV Extent row_extent(const AttendParams& p, int32_t s) {
   e.n = akv_held(p.tab, p.kv.bs_log2, s);
   e.lo = p.window > 0 && e.n > p.window ? e.n - p.window : 0;
   if (p.selected) {
-    const int64_t blocks = (static_cast<int64_t>(e.n) + (1 << p.kv.bs_log2) - 1) >> p.kv.bs_log2;
-    const int64_t taken = (blocks < p.keep ? blocks : p.keep) << p.kv.bs_log2;
+    const int32_t blocks = (e.n + (1 << p.kv.bs_log2) - 1) >> p.kv.bs_log2;
+    const int32_t taken = (blocks < p.keep ? blocks : p.keep) << p.kv.bs_log2;
     e.first = 0;
-    e.chunks = static_cast<int32_t>((taken + kChunk - 1) / kChunk);
+    e.chunks = (taken + kChunk - 1) / kChunk;
   } else {
     e.first = e.lo / kChunk;
-    e.chunks = static_cast<int32_t>((static_cast<int64_t>(e.n) + kChunk - 1) / kChunk) - e.first;
+    e.chunks = (e.n + kChunk - 1) / kChunk - e.first;
   }
   return e;
 }
 
-// A warp's view of the blocks under its tiles: lane i holds one table entry,
-// for the next 32 (or fewer, where a tile spans several blocks) tiles.
-struct Cursor {
-  int32_t id, place;  // this lane's block (-1: none) and its place in the table
-  int32_t from;       // the first chunk that the entries are for
+// A run of positions that lie behind one another in one block: 8, or 1 where
+// blocks are smaller.
+struct Run {
+  int32_t id;   // the block, kNone: none
+  int32_t pos;  // the first position
+  static constexpr int32_t kNone = INT_MIN;
+};
 
-  AKV_DEV static int entries(int bs_log2) { return bs_log2 >= 4 ? 1 : 16 >> bs_log2; }
+// The run at token `tok` of the row's list (of its selected blocks, where there is a
+// selection).
+AKV_DEV Run find_run(const AttendParams& p, const Extent& e, int32_t s, int32_t h, int32_t tok) {
+  const int bl = p.kv.bs_log2;
+  const int32_t blocks = (e.n + (1 << bl) - 1) >> bl;
+  Run run = {Run::kNone, 0};
+  int32_t place = tok >> bl;
+  if (place >= blocks) return run;
+  if (p.selected) {
+    if (place >= p.keep) return run;
+    place = p.selected[(static_cast<int64_t>(s) * p.kv.heads + h) * p.keep + place];
+    if (place < -1 || place >= blocks) akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, place, blocks);
+    if (place < 0 || place >= blocks) return run;
+  }
+  if (((place + 1ll) << bl) <= e.lo) return run;
+  run.pos = (place << bl) + (tok & ((1 << bl) - 1));
+  run.id = p.tab.ids[s * p.tab.stride + place];
+  return run;
+}
+
+// The block of a run, if the pool has it.
+AKV_DEV bool run_ok(const AttendParams& p, const Run& run, int32_t s) {
+  if (static_cast<uint32_t>(run.id) < static_cast<uint32_t>(p.kv.total)) return true;
+  if (run.id != Run::kNone) akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, run.id, p.kv.total);
+  return false;
+}
+
+// Which of the `count` positions from `pos` take part.
+AKV_DEV uint32_t taking_part(const Extent& e, int32_t pos, int count) {
+  const int low = max(0, min(count, e.lo - pos)), high = max(low, min(count, e.n - pos));
+  return ((1u << high) - 1) & ~((1u << low) - 1);
+}
+
+// A warp's view of the runs under its tiles: lane i holds where one lies, for
+// the next 16 (or 2) tiles.
+struct Cursor {
+  int64_t off;    // bytes from the layer's K of this head
+  uint32_t part;  // which of the run's positions take part
+  uint32_t full;  // bit i: all of lane i's run does
+  int32_t from;   // the first chunk that the runs are for
+
+  AKV_DEV static int run_log2(int bs_log2) { return bs_log2 >= 3 ? 3 : 0; }
+  AKV_DEV static int runs(int bs_log2) { return kTile >> run_log2(bs_log2); }  // per tile
 
   AKV_DEV void refill(const AttendParams& p, const Extent& e, int32_t s, int32_t h, int32_t chunk, int32_t end,
                       int warp, int lane) {
     from = chunk;
-    const int bl = p.kv.bs_log2, per = entries(bl);
-    const int64_t c = static_cast<int64_t>(chunk) + lane / per;
-    const int64_t tok = c * kChunk + warp * kTile + (static_cast<int64_t>(lane % per) << bl);
-    const int64_t vb = tok >> bl;
-    const int64_t blocks = (static_cast<int64_t>(e.n) + (1 << bl) - 1) >> bl;
-    id = -1;
-    place = -1;
-    if (c >= end) return;
-    if (p.selected) {
-      if (vb >= p.keep || vb >= blocks) return;
-      place = p.selected[(static_cast<int64_t>(s) * p.kv.heads + h) * p.keep + vb];
-      if (place < -1 || place >= blocks) {
-        akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, place, static_cast<int32_t>(blocks));
-        place = -1;
-      }
-      if (place < 0 || ((static_cast<int64_t>(place) + 1) << bl) <= e.lo) return;
-    } else {
-      if (vb >= blocks || ((vb + 1) << bl) <= e.lo) return;
-      place = static_cast<int32_t>(vb);
-    }
-    id = p.tab.ids[s * p.tab.stride + place];
-    if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.kv.total)) {
-      akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, id, p.kv.total);
-      id = -1;
-    }
+    const int bl = p.kv.bs_log2, rl = run_log2(bl), per = runs(bl);
+    const int32_t c = chunk + lane / per;
+    Run run = {Run::kNone, 0};
+    if (c < end) run = find_run(p, e, s, h, c * kChunk + warp * kTile + (lane % per << rl));
+    const bool ok = run_ok(p, run, s);
+    off = ok ? run.id * p.kv.page_bytes + static_cast<int64_t>(run.pos & ((1 << bl) - 1)) * p.kv.row_bytes : 0;
+    part = ok ? taking_part(e, run.pos, 1 << rl) : 0;
+    full = __ballot_sync(kFullWarp, part == (1u << (1 << rl)) - 1);
   }
-  // The lane that holds the entry of position r (0..15) of chunk's tile.
+  // The lane that holds the run of position r (0..15) of chunk's tile.
   AKV_DEV int lane_of(int bs_log2, int32_t chunk, int r) const {
-    return (chunk - from) * entries(bs_log2) + (bs_log2 >= 4 ? 0 : r >> bs_log2);
+    return (chunk - from) * runs(bs_log2) + (r >> run_log2(bs_log2));
   }
-  AKV_DEV bool covers(int bs_log2, int32_t chunk) const { return (chunk - from + 1) * entries(bs_log2) <= 32; }
-
-  // Which of the tile's 16 positions take part (bit r), and the tile's first
-  // position within its block (its rows lie behind one another there).
-  AKV_DEV uint32_t valid(const AttendParams& p, const Extent& e, int32_t chunk, int warp, int lane) const {
-    const int bl = p.kv.bs_log2, r = lane & 15;
-    const int src = lane_of(bl, chunk, r);
-    const int32_t b = __shfl_sync(kFullWarp, id, src);
-    const int32_t at = __shfl_sync(kFullWarp, place, src);
-    const int32_t in = (chunk * kChunk + warp * kTile + r) & ((1 << bl) - 1);
-    const int64_t pos = (static_cast<int64_t>(at) << bl) + in;
-    const bool ok = b >= 0 && pos >= e.lo && pos < e.n;
-    return __ballot_sync(kFullWarp, ok) & 0xffffu;
+  AKV_DEV bool covers(int bs_log2, int32_t chunk) const { return (chunk - from + 1) * runs(bs_log2) <= 32; }
+  // Where position r of chunk's tile lies (all lanes call).
+  AKV_DEV int64_t row(const AttendParams& p, int32_t chunk, int r) const {
+    const int bl = p.kv.bs_log2, in = r & ((1 << run_log2(bl)) - 1);
+    return __shfl_sync(kFullWarp, off, lane_of(bl, chunk, r)) + in * p.kv.row_bytes;
+  }
+  // Which of the tile's 16 positions take part (bit r).
+  AKV_DEV uint32_t valid(const AttendParams& p, int32_t chunk, int lane) const {
+    const int bl = p.kv.bs_log2, r = lane & 15, per = runs(bl);
+    const uint32_t mine = full >> (chunk - from) * per;
+    if (per == 2 && (mine & 3) == 3) return 0xffff;
+    const uint32_t bits = __shfl_sync(kFullWarp, part, lane_of(bl, chunk, r));
+    return __ballot_sync(kFullWarp, bits >> (r & ((1 << run_log2(bl)) - 1)) & 1) & 0xffff;
   }
 };
 
@@ -147,8 +176,12 @@ struct Cursor {
 // is free, so each lane loads 16 consecutive bytes of a row and the products
 // take them in that order (lane 4 g + c holds dimensions 32 i + 8 c .. + 7 of
 // key rows g and g + 8; of V, dimensions 64 i + 8 g .. + 7 of positions 2 c,
-// 2 c + 1, 2 c + 8, 2 c + 9).  The next tile's keys are loaded as soon as this one's have been
-// used, this one's values while the scores are computed.
+// 2 c + 1, 2 c + 8, 2 c + 9).  The next tile's keys are loaded as soon as this
+// one's have been used, this one's values while the scores are computed.
+// (Measured on 256 rows of 4,096 positions, 4.3 GB, where a plain read of the
+// same blocks takes 615 us: 16-byte asynchronous copies into shared memory
+// 846 us, bulk copies of whole blocks 765 us: their issue and the reads
+// from shared memory held the warps up more than the memory did.)
 template <typename T>
 struct Pack2;
 template <>
@@ -160,8 +193,7 @@ struct Pack2<__half> {
   AKV_DEV static float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
   AKV_DEV static void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                           uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
@@ -175,8 +207,7 @@ struct Pack2<__nv_bfloat16> {
   AKV_DEV static float2 unpack(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
   AKV_DEV static void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                           uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
@@ -184,7 +215,7 @@ struct Pack2<__nv_bfloat16> {
 
 AKV_DEV uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 
@@ -194,7 +225,6 @@ AKV_DEV float exp2_fast(float x) {
   return y;
 }
 
-// Streaming loads: a block is read once per launch.
 AKV_DEV uint4 ld16(const char* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 AKV_DEV uint2 ld8(const char* p) { return __ldg(reinterpret_cast<const uint2*>(p)); }
 
@@ -202,7 +232,7 @@ template <typename T, int kD, int kN>
 struct MmaEngine {
   using Type = T;
   static constexpr int kDim = kD;          // compiled for this head dim
-  static constexpr int kHeads = 8 * kN;    // query heads per pair
+  static constexpr int kCols = 8 * kN;     // query heads per pair
   static constexpr int kCtas = kD <= 128 && kN == 1 ? 3 : (kD <= 128 ? 2 : 1);
   static constexpr int kKi = kD / 32;      // 16-byte words of a key row per lane
   static constexpr int kVi = kD / 64;      // the same of a value row,
@@ -211,19 +241,25 @@ struct MmaEngine {
 
   uint4 q[kN][kKi];
   uint4 ka[kKi], kb[kKi];
-  uint4 v[4][kVi > 0 ? kVi : 1];
+  uint4 v[4][kVi];
   uint2 vr[4];
   float o[kN][kMt][4];
   float m[kN][2], l[kN][2];
 
-  AKV_DEV void load_k(const AttendParams& p, const Cursor& cur, const char* kbase, int32_t chunk, uint32_t vm, int warp,
+  // Positions that take no part (bits of vm) are 0, whatever the block holds.
+  AKV_DEV void load_k(const AttendParams& p, const Cursor& cur, const char* base, int32_t chunk, uint32_t vm,
                       int lane) {
-    const int g = lane >> 2, c = lane & 3, bl = p.kv.bs_log2;
-    const int32_t ida = __shfl_sync(kFullWarp, cur.id, cur.lane_of(bl, chunk, g));
-    const int32_t idb = __shfl_sync(kFullWarp, cur.id, cur.lane_of(bl, chunk, g + 8));
-    const int32_t t0 = chunk * kChunk + warp * kTile, mask = (1 << bl) - 1;
-    const char* pa = kbase + ida * p.kv.page_bytes + ((t0 + g) & mask) * (kD * 2) + c * 16;
-    const char* pb = kbase + idb * p.kv.page_bytes + ((t0 + g + 8) & mask) * (kD * 2) + c * 16;
+    const int g = lane >> 2, c = lane & 3;
+    const char *pa, *pb;
+    if (p.kv.bs_log2 >= 3) {
+      pa = base + __shfl_sync(kFullWarp, cur.off, (chunk - cur.from) * 2) + g * (kD * 2);
+      pb = base + __shfl_sync(kFullWarp, cur.off, (chunk - cur.from) * 2 + 1) + g * (kD * 2);
+    } else {
+      pa = base + cur.row(p, chunk, g);
+      pb = base + cur.row(p, chunk, g + 8);
+    }
+    pa += c * 16;
+    pb += c * 16;
     if (vm == 0xffffu) {
 #pragma unroll
       for (int i = 0; i < kKi; ++i) {
@@ -240,20 +276,27 @@ struct MmaEngine {
     }
   }
 
-  // Values of positions that take no part are 0, whatever the block holds.
-  AKV_DEV void load_v(const AttendParams& p, const Cursor& cur, const char* vbase, int32_t chunk, uint32_t vm, int warp,
+  AKV_DEV void load_v(const AttendParams& p, const Cursor& cur, const char* base, int32_t chunk, uint32_t vm,
                       int lane) {
-    const int g = lane >> 2, c = lane & 3, bl = p.kv.bs_log2;
-    const int32_t t0 = chunk * kChunk + warp * kTile, mask = (1 << bl) - 1;
+    const int g = lane >> 2, c = lane & 3;
+    const char* row[4];
+    if (p.kv.bs_log2 >= 3) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        row[2 * half] = base + __shfl_sync(kFullWarp, cur.off, (chunk - cur.from) * 2 + half) + c * (kD * 4);
+        row[2 * half + 1] = row[2 * half] + kD * 2;
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) row[x] = base + cur.row(p, chunk, 2 * c + (x & 1) + (x >> 1) * 8);
+    }
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int r = 2 * c + (x & 1) + (x >> 1) * 8;
-      const int32_t id = __shfl_sync(kFullWarp, cur.id, cur.lane_of(bl, chunk, r));
-      const char* pv = vbase + id * p.kv.page_bytes + ((t0 + r) & mask) * (kD * 2);
       if (vm == 0xffffu || ((vm >> r) & 1)) {
 #pragma unroll
-        for (int i = 0; i < kVi; ++i) v[x][i] = ld16(pv + i * 128 + g * 16);
-        if (kVr) vr[x] = ld8(pv + kVi * 128 + g * 8);
+        for (int i = 0; i < kVi; ++i) v[x][i] = ld16(row[x] + i * 128 + g * 16);
+        if (kVr) vr[x] = ld8(row[x] + kVi * 128 + g * 8);
       } else {
 #pragma unroll
         for (int i = 0; i < kVi; ++i) v[x][i] = make_uint4(0, 0, 0, 0);
@@ -267,23 +310,22 @@ struct MmaEngine {
     const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
     const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      Pack2<T>::mma(o[n][tile], a0, a1, a2, a3, hi[n][0], hi[n][1]);
-      Pack2<T>::mma(o[n][tile], a0, a1, a2, a3, lo[n][0], lo[n][1]);
-    }
+    for (int n = 0; n < kN; ++n) Pack2<T>::mma(o[n][tile], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+#pragma unroll
+    for (int n = 0; n < kN; ++n) Pack2<T>::mma(o[n][tile], a0, a1, a2, a3, lo[n][0], lo[n][1]);
   }
 
-  // Chunks [a, b) of pair (s, h, part).
-  AKV_DEV void run(const AttendParams& p, const Extent& e, int32_t s, int32_t h, int32_t part, int32_t a, int32_t b,
+  // Chunks [a, b) of pair (s, h, part): this warp's tiles.
+  AKV_DEV void run(const AttendParams& p, const Extent& ext, int32_t s, int32_t h, int32_t part, int32_t a, int32_t b,
                    int warp, int lane) {
     const int g = lane >> 2, c = lane & 3;
     const char* kbase = p.kv.base + h * p.kv.tile_bytes;
     const char* vbase = kbase + p.kv.kv_bytes;
     Cursor cur;
-    cur.refill(p, e, s, h, a, b, warp, lane);
+    cur.refill(p, ext, s, h, a, b, warp, lane);
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      const int32_t head = part * kHeads + n * 8 + g;
+      const int32_t head = part * kCols + n * 8 + g;
       const T* row = static_cast<const T*>(p.q) + s * p.q_row + (static_cast<int64_t>(h) * p.group + head) * p.q_head;
 #pragma unroll
       for (int i = 0; i < kKi; ++i)
@@ -292,51 +334,56 @@ struct MmaEngine {
       for (int t = 0; t < kMt; ++t)
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[n][t][x] = 0.f;
-      m[n][0] = m[n][1] = -INFINITY;
+      m[n][0] = m[n][1] = kLowest;
       l[n][0] = l[n][1] = 0.f;
     }
-    uint32_t vm = cur.valid(p, e, a, warp, lane);
-    load_k(p, cur, kbase, a, vm, warp, lane);
+    uint32_t vm = cur.valid(p, a, lane);
+    load_k(p, cur, kbase, a, vm, lane);
     for (int32_t chunk = a; chunk < b; ++chunk) {
-      load_v(p, cur, vbase, chunk, vm, warp, lane);
+      load_v(p, cur, vbase, chunk, vm, lane);
       float sc[kN][4];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
+        float odd[4] = {0.f, 0.f, 0.f, 0.f};  // two chains of products
         sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < kKi; ++i) {
           Pack2<T>::mma(sc[n], ka[i].x, kb[i].x, ka[i].y, kb[i].y, q[n][i].x, q[n][i].y);
-          Pack2<T>::mma(sc[n], ka[i].z, kb[i].z, ka[i].w, kb[i].w, q[n][i].z, q[n][i].w);
+          Pack2<T>::mma(odd, ka[i].z, kb[i].z, ka[i].w, kb[i].w, q[n][i].z, q[n][i].w);
         }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[n][x] += odd[x];
       }
       const uint32_t now = vm;
       if (chunk + 1 < b) {
-        if (!cur.covers(p.kv.bs_log2, chunk + 1)) cur.refill(p, e, s, h, chunk + 1, b, warp, lane);
-        vm = cur.valid(p, e, chunk + 1, warp, lane);
-        load_k(p, cur, kbase, chunk + 1, vm, warp, lane);
+        if (!cur.covers(p.kv.bs_log2, chunk + 1)) cur.refill(p, ext, s, h, chunk + 1, b, warp, lane);
+        vm = cur.valid(p, chunk + 1, lane);
+        load_k(p, cur, kbase, chunk + 1, vm, lane);
       }
-      bool raise = false;
+      float e[kN][4], above = 0.f;
+      auto exponents = [&]() {
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          sc[n][x] *= p.scale_log2;
-          if (!((now >> (g + (x >> 1) * 8)) & 1)) sc[n][x] = -INFINITY;
-        }
-        raise |= fmaxf(sc[n][0], sc[n][2]) > m[n][0] + kLazy;
-        raise |= fmaxf(sc[n][1], sc[n][3]) > m[n][1] + kLazy;
-      }
-      if (__any_sync(kFullWarp, raise)) {
+          for (int x = 0; x < 4; ++x) {
+            e[n][x] = fmaf(sc[n][x], p.scale_log2, -m[n][x & 1]);
+            if (now != 0xffff && !(now >> (g + (x >> 1) * 8) & 1)) e[n][x] = -INFINITY;
+            above = fmaxf(above, e[n][x]);
+          }
+      };
+      exponents();
+      if (__any_sync(kFullWarp, above > kLazy)) {
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float top = fmaxf(sc[n][x], sc[n][x + 2]);
+            float top = m[n][x];
+            if (now >> g & 1) top = fmaxf(top, sc[n][x] * p.scale_log2);
+            if (now >> (g + 8) & 1) top = fmaxf(top, sc[n][x + 2] * p.scale_log2);
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, off));
-            const float to = fmaxf(m[n][x], top);
-            const float by = to == -INFINITY ? 1.f : exp2_fast(m[n][x] - to);
-            m[n][x] = to;
+            const float by = exp2_fast(m[n][x] - top);
+            m[n][x] = top;
             l[n][x] *= by;
 #pragma unroll
             for (int t = 0; t < kMt; ++t) {
@@ -344,6 +391,7 @@ struct MmaEngine {
               o[n][t][x + 2] *= by;
             }
           }
+        exponents();
       }
       // The weights go into the product as the sum of two 16-bit numbers:
       // one alone would be off by half a step of the type, as much as the
@@ -351,10 +399,9 @@ struct MmaEngine {
       uint32_t hi[kN][2], lo[kN][2];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float w0 = exp2_fast(sc[n][2 * x] - m0), w1 = exp2_fast(sc[n][2 * x + 1] - m1);
+          const float w0 = exp2_fast(e[n][2 * x]), w1 = exp2_fast(e[n][2 * x + 1]);
           l[n][0] += w0;
           l[n][1] += w1;
           const uint32_t top = Pack2<T>::pack(w0, w1);
@@ -377,7 +424,7 @@ struct MmaEngine {
     }
   }
 
-  // This warp's sums: acc [kHeads][kD], and m and l of each head.
+  // This warp's sums: acc [kCols][kD], and m and l of each head.
   AKV_DEV void store(float* acc, float2* ml, int /*dim*/, int lane) {
     const int g = lane >> 2, c = lane & 3;
 #pragma unroll
@@ -399,148 +446,190 @@ struct MmaEngine {
 };
 
 // ── 32-bit engine: any type and head dim (up to 256) ───────────────────────
-// Multiplies and adds in 32 bits.  A lane holds kE consecutive dimensions of
-// every 32 kE; 4 positions at a time give 4 * kHeads partial scores per lane,
-// which halving exchanges turn into one whole score (or a copy) per lane.
-template <typename T, int kE, int kJ, int kH>
+// Multiplies and adds in 32 bits, one row per pair.  kL lanes hold a row
+// between them, kE consecutive dimensions of every kL kE each, so a warp has
+// 32 / kL positions at a time; kU such steps give kU * kH partial scores per
+// lane, which halving exchanges turn into one whole score (or a copy) per
+// lane.  The next positions are loaded while these are computed.
+template <typename T, int kE, int kJ, int kL, int kH>
 struct SimtEngine {
   using Type = T;
   static constexpr int kDim = 0;
-  static constexpr int kHeads = kH;
-  static constexpr int kCtas = kH * kE * kJ >= 64 ? 2 : 3;
-  static constexpr int kX = kE * kJ;       // dimensions per lane
-  static constexpr int kU = 4;             // positions at a time
-  static constexpr int kVals = kU * kH;    // scores at a time,
-  static constexpr int kStep = 32 / kVals;  // each held by this many lanes
+  static constexpr int kCols = kH;
+  static constexpr int kX = kE * kJ;                      // dimensions per lane
+  static constexpr int kCtas = kH * kX * kL >= 32 * 32 ? 2 : 3;
+  static constexpr int kSub = 32 / kL;                    // positions at a time
+  static constexpr int kU = kL / kH < 4 || kX > 4 ? 2 : 4;
+  static constexpr int kVals = kU * kH;                   // scores at a time,
+  static constexpr int kStep = kL / kVals;                // each held by this many lanes
+  static constexpr int kPass = kU * kSub;                 // positions of a pass
+  static_assert(kTile % kPass == 0 && kStep >= 1, "a tile is whole passes");
   using Vec = AkvVec<T, kE>;
 
   float q[kH][kX], o[kH][kX];
-  float m, l;  // of this lane's head, l over this lane's position of each four
+  float m, l;  // of this lane's head, l over this lane's positions
 
-  AKV_DEV static void load_row(float (&x)[kX], const char* row, int dim, bool ok, int lane) {
+  AKV_DEV static Vec zero() {
+    Vec w;
+#pragma unroll
+    for (int i = 0; i < kE; ++i) w.v[i] = from_f32<T>(0.f);
+    return w;
+  }
+  AKV_DEV static void load_row(Vec (&x)[kJ], const char* row, int dim, bool ok, int at) {
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
-      const int d = (j * 32 + lane) * kE;
-      if (ok && d < dim) {
-        const Vec w = *reinterpret_cast<const Vec*>(row + d * sizeof(T));
-#pragma unroll
-        for (int i = 0; i < kE; ++i) x[j * kE + i] = to_f32<T>(w.v[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kE; ++i) x[j * kE + i] = 0.f;
-      }
+      const int d = (j * kL + at) * kE;
+      x[j] = ok && d < dim ? *reinterpret_cast<const Vec*>(row + d * sizeof(T)) : zero();
     }
   }
 
+  AKV_DEV void load_pass(const AttendParams& p, const Cursor& cur, const char* kbase, int32_t chunk, uint32_t vm,
+                         int r0, int lane, Vec (&k)[kU][kJ], Vec (&v)[kU][kJ]) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int r = r0 + u * kSub + lane / kL;
+      const char* row = kbase + cur.row(p, chunk, r);
+      load_row(k[u], row, p.kv.dim, (vm >> r) & 1, lane % kL);
+      load_row(v[u], row + p.kv.kv_bytes, p.kv.dim, (vm >> r) & 1, lane % kL);
+    }
+  }
+
+  AKV_DEV void compute(const AttendParams& p, uint32_t vm, int r0, int lane, const Vec (&k)[kU][kJ],
+                       const Vec (&v)[kU][kJ]) {
+    const int at = lane % kL, mine = at / kStep % kU;  // this lane's position of the kU
+    float val[kVals];
+#pragma unroll
+    for (int n = 0; n < kH; ++n)
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        float d = 0.f;
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
+#pragma unroll
+          for (int i = 0; i < kE; ++i) d = fmaf(q[n][j * kE + i], to_f32<T>(k[u][j].v[i]), d);
+        val[n * kU + u] = d;
+      }
+    // value i ends, whole, in lanes i * kStep ..: each exchange keeps the
+    // half of the values that belongs to this lane's half
+    int off = kL / 2;
+#pragma unroll
+    for (int w = kVals / 2; w >= 1; w >>= 1, off >>= 1) {
+      const bool up = lane & off;
+#pragma unroll
+      for (int i = 0; i < w; ++i) {
+        const float send = up ? val[i] : val[i + w];
+        const float keep = up ? val[i + w] : val[i];
+        val[i] = keep + __shfl_xor_sync(kFullWarp, send, off);
+      }
+    }
+#pragma unroll
+    for (int x = kStep / 2; x >= 1; x >>= 1) val[0] += __shfl_xor_sync(kFullWarp, val[0], x);
+    const bool in = (vm >> (r0 + mine * kSub + lane / kL)) & 1;
+    const float sc = val[0] * p.scale_log2;
+    if (__any_sync(kFullWarp, in && sc > m + kLazy)) {
+      float top = in ? fmaxf(sc, m) : m;
+#pragma unroll
+      for (int x = kStep; x < kStep * kU; x <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, x));
+#pragma unroll
+      for (int x = kL; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, x));
+      const float by = exp2f(m - top);
+      m = top;
+      l *= by;
+#pragma unroll
+      for (int n = 0; n < kH; ++n) {
+        const float f = __shfl_sync(kFullWarp, by, n * kU * kStep);
+#pragma unroll
+        for (int x = 0; x < kX; ++x) o[n][x] *= f;
+      }
+    }
+    const float w = in ? exp2f(sc - m) : 0.f;
+    l += w;
+#pragma unroll
+    for (int n = 0; n < kH; ++n)
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const float f = __shfl_sync(kFullWarp, w, (lane & ~(kL - 1)) + (n * kU + u) * kStep);
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
+#pragma unroll
+          for (int i = 0; i < kE; ++i) o[n][j * kE + i] = fmaf(f, to_f32<T>(v[u][j].v[i]), o[n][j * kE + i]);
+      }
+  }
+
+  // Chunks [a, b) of pair (s, h, part): this warp's tiles.
   AKV_DEV void run(const AttendParams& p, const Extent& e, int32_t s, int32_t h, int32_t part, int32_t a, int32_t b,
                    int warp, int lane) {
-    const char* kbase = p.kv.base + h * p.kv.tile_bytes;
-    const char* vbase = kbase + p.kv.kv_bytes;
-    const int bl = p.kv.bs_log2, mask = (1 << bl) - 1;
-    Cursor cur;
-    cur.refill(p, e, s, h, a, b, warp, lane);
 #pragma unroll
     for (int n = 0; n < kH; ++n) {
       const int32_t head = part * kH + n;
       const T* row = static_cast<const T*>(p.q) + s * p.q_row + (static_cast<int64_t>(h) * p.group + head) * p.q_head;
-      load_row(q[n], reinterpret_cast<const char*>(row), p.kv.dim, head < p.group, lane);
+      Vec w[kJ];
+      load_row(w, reinterpret_cast<const char*>(row), p.kv.dim, head < p.group, lane % kL);
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+#pragma unroll
+        for (int i = 0; i < kE; ++i) q[n][j * kE + i] = to_f32<T>(w[j].v[i]);
 #pragma unroll
       for (int x = 0; x < kX; ++x) o[n][x] = 0.f;
     }
-    m = -INFINITY;
+    m = kLowest;
     l = 0.f;
-    const int mine = lane / kStep % kU;  // this lane's position of each four
+    const char* kbase = p.kv.base + h * p.kv.tile_bytes;
+    Cursor cur;
+    cur.refill(p, e, s, h, a, b, warp, lane);
+    uint32_t vm = cur.valid(p, a, lane);
+    Vec k[kU][kJ], v[kU][kJ];
+    load_pass(p, cur, kbase, a, vm, 0, lane, k, v);
     for (int32_t chunk = a; chunk < b; ++chunk) {
-      if (!cur.covers(bl, chunk)) cur.refill(p, e, s, h, chunk, b, warp, lane);
-      const uint32_t vm = cur.valid(p, e, chunk, warp, lane);
-      if (vm == 0) continue;
-      const int32_t t0 = chunk * kChunk + warp * kTile;
 #pragma unroll 1
-      for (int r0 = 0; r0 < kTile; r0 += kU) {
-        float k[kU][kX], v[kU][kX];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const int r = r0 + u;
-          const int32_t id = __shfl_sync(kFullWarp, cur.id, cur.lane_of(bl, chunk, r));
-          const int64_t off = id * p.kv.page_bytes + static_cast<int64_t>((t0 + r) & mask) * p.kv.row_bytes;
-          load_row(k[u], kbase + off, p.kv.dim, (vm >> r) & 1, lane);
-          load_row(v[u], vbase + off, p.kv.dim, (vm >> r) & 1, lane);
+      for (int r0 = 0; r0 < kTile; r0 += kPass) {
+        Vec kn[kU][kJ], vn[kU][kJ];
+        const uint32_t now = vm;
+        const bool last = r0 + kPass >= kTile, more = !last || chunk + 1 < b;
+        if (last && more) {
+          if (!cur.covers(p.kv.bs_log2, chunk + 1)) cur.refill(p, e, s, h, chunk + 1, b, warp, lane);
+          vm = cur.valid(p, chunk + 1, lane);
         }
-        float val[kVals];
+        if (more) load_pass(p, cur, kbase, last ? chunk + 1 : chunk, vm, last ? 0 : r0 + kPass, lane, kn, vn);
+        if (now >> r0 & ((1u << kPass) - 1)) compute(p, now, r0, lane, k, v);
+        if (more) {
 #pragma unroll
-        for (int n = 0; n < kH; ++n)
+          for (int u = 0; u < kU; ++u)
 #pragma unroll
-          for (int u = 0; u < kU; ++u) {
-            float d = 0.f;
-#pragma unroll
-            for (int x = 0; x < kX; ++x) d = fmaf(q[n][x], k[u][x], d);
-            val[n * kU + u] = d;
-          }
-        // value i ends, whole, in lanes i * kStep ..: each exchange keeps
-        // the half of the values that belongs to this lane's half
-        int off = 16;
-#pragma unroll
-        for (int w = kVals / 2; w >= 1; w >>= 1, off >>= 1) {
-          const bool up = lane & off;
-#pragma unroll
-          for (int i = 0; i < w; ++i) {
-            const float send = up ? val[i] : val[i + w];
-            const float keep = up ? val[i + w] : val[i];
-            val[i] = keep + __shfl_xor_sync(kFullWarp, send, off);
-          }
+            for (int j = 0; j < kJ; ++j) {
+              k[u][j] = kn[u][j];
+              v[u][j] = vn[u][j];
+            }
         }
-#pragma unroll
-        for (int x = kStep / 2; x >= 1; x >>= 1) val[0] += __shfl_xor_sync(kFullWarp, val[0], x);
-        const bool in = (vm >> (r0 + mine)) & 1;
-        const float sc = in ? val[0] * p.scale_log2 : -INFINITY;
-        if (__any_sync(kFullWarp, sc > m + kLazy)) {
-          float top = sc;
-          top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, kStep));
-          top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, 2 * kStep));
-          const float to = fmaxf(m, top);
-          const float by = to == -INFINITY ? 1.f : exp2f(m - to);
-          m = to;
-          l *= by;
-#pragma unroll
-          for (int n = 0; n < kH; ++n) {
-            const float f = __shfl_sync(kFullWarp, by, n * kU * kStep);
-#pragma unroll
-            for (int x = 0; x < kX; ++x) o[n][x] *= f;
-          }
-        }
-        const float w = exp2f(sc - (m == -INFINITY ? 0.f : m));
-        l += w;
-#pragma unroll
-        for (int n = 0; n < kH; ++n)
-#pragma unroll
-          for (int u = 0; u < kU; ++u) {
-            const float f = __shfl_sync(kFullWarp, w, (n * kU + u) * kStep);
-#pragma unroll
-            for (int x = 0; x < kX; ++x) o[n][x] = fmaf(f, v[u][x], o[n][x]);
-          }
       }
     }
   }
 
   AKV_DEV void store(float* acc, float2* ml, int dim, int lane) {
     float sum = l;
-    sum += __shfl_xor_sync(kFullWarp, sum, kStep);
-    sum += __shfl_xor_sync(kFullWarp, sum, 2 * kStep);
-    if (lane % (kU * kStep) == 0) ml[lane / (kU * kStep)] = make_float2(m, sum);
+#pragma unroll
+    for (int x = kStep; x < kStep * kU; x <<= 1) sum += __shfl_xor_sync(kFullWarp, sum, x);
+#pragma unroll
+    for (int x = kL; x < 32; x <<= 1) sum += __shfl_xor_sync(kFullWarp, sum, x);
+    if (lane < kL && lane % (kU * kStep) == 0) ml[lane / (kU * kStep)] = make_float2(m, sum);
 #pragma unroll
     for (int n = 0; n < kH; ++n)
 #pragma unroll
       for (int j = 0; j < kJ; ++j)
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
-          const int d = (j * 32 + lane) * kE + i;
-          if (d < dim) acc[n * dim + d] = o[n][j * kE + i];
+          float x = o[n][j * kE + i];
+#pragma unroll
+          for (int w = kL; w < 32; w <<= 1) x += __shfl_xor_sync(kFullWarp, x, w);
+          const int d = (j * kL + lane % kL) * kE + i;
+          if (d < dim && lane < kL) acc[n * dim + d] = x;
         }
   }
 };
 
-// The factor that brings sums taken with maximum m to maximum `to` (both may be -inf: no sums).
-AKV_DEV float join_factor(float m, float to) { return m == -INFINITY ? 0.f : exp2f(m - to); }
+// The factor that brings sums taken with maximum ml.x to maximum `to`; nothing
+// (ml.y == 0) stays nothing.
+AKV_DEV float join_factor(float2 ml, float to) { return ml.y == 0.f ? 0.f : exp2f(ml.x - to); }
 
 template <typename T>
 AKV_DEV void finish(const AttendParams& p, int32_t s, int32_t head, int d, float o, float l) {
@@ -553,49 +642,57 @@ AKV_DEV void finish_lse(const AttendParams& p, int32_t s, int32_t head, float m,
     p.lse[static_cast<int64_t>(s) * p.kv.heads * p.group + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-AKV_HD int64_t piece_floats(int heads, int dim) { return static_cast<int64_t>(heads) * (dim + 2); }
+// A piece: [cols][dim] sums, then [cols] (m, l).
+AKV_HD int64_t piece_floats(int cols, int dim) { return (static_cast<int64_t>(cols) * (dim + 2) + 3) / 4 * 4; }
+
+// What a launch's CTAs agree on: unit u of `total` belongs to CTA cta_of(u).
+struct Deal {
+  int64_t total, ctas;
+  AKV_DEV int64_t begin(int64_t c) const { return total * c / ctas; }
+  AKV_DEV int64_t cta_of(int64_t u) const {
+    int64_t c = u * ctas / total;
+    while (begin(c + 1) <= u) ++c;
+    while (begin(c) > u) --c;
+    return c;
+  }
+};
 
 template <class Eng>
 __global__ void __launch_bounds__(kThreads, Eng::kCtas) k_attend(AttendParams p) {
   using T = typename Eng::Type;
-  constexpr int kH = Eng::kHeads;
+  constexpr int kC = Eng::kCols;
   using Search = AkvRowSearch<kThreads>;
-  extern __shared__ __align__(16) float acc[];  // [kWarps][kH][dim]
-  __shared__ float2 ml[kWarps][kH];
-  __shared__ float factor[kWarps][kH];
-  __shared__ float2 joined[kH];
+  extern __shared__ __align__(16) float acc[];  // [kWarps][kC][dim]
+  __shared__ float2 ml[kWarps][kC];
+  __shared__ float factor[kWarps][kC];
+  __shared__ float2 joined[kC];
+  __shared__ int32_t order;  // of this CTA's arrival
   __shared__ typename Search::Shared sh;
-  akv_grid_release();  // k_join may take its place; it waits for this grid's end
-  if (akv_failed(p.st)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int dim = Eng::kDim ? Eng::kDim : p.kv.dim;
   const int64_t pairs = static_cast<int64_t>(p.kv.heads) * p.parts;  // of a row
   auto units = [&](int32_t s) -> int64_t { return row_extent(p, s).chunks * pairs; };
 
   int32_t s = 0;
-  int64_t rest = 0, x = 0, end = 0, total = 0, ctas = gridDim.x;
-  AttendMeta meta = {0, 0, 0, 0};
-  if (p.direct) {
-    s = static_cast<int32_t>(blockIdx.x / pairs);
-    const int32_t chunks = row_extent(p, s).chunks;
-    rest = blockIdx.x % pairs * chunks;
-    end = chunks;
-  } else {
+  int64_t rest = 0, x = 0, end = 0;
+  Deal deal;
+  {
     Search search;
     search.scan(sh, p.tab.rows, units);
-    total = search.total;
-    if (ctas > total) ctas = total;
-    if (blockIdx.x < ctas) {
-      x = total * blockIdx.x / ctas;
-      end = total * (blockIdx.x + 1) / ctas;
+    deal.total = search.total;
+    deal.ctas = gridDim.x < deal.total ? gridDim.x : deal.total;
+    if (blockIdx.x < deal.ctas) {
+      x = deal.begin(blockIdx.x);
+      end = deal.begin(blockIdx.x + 1);
       search.find(sh, x, units, s, rest);
     }
   }
   // rows that hold nothing, and lengths that the table cannot hold
   for (int32_t r = blockIdx.x; r < p.tab.rows; r += gridDim.x) {
-    if (threadIdx.x == 0 && p.tab.lengths[r] > akv_held(p.tab, p.kv.bs_log2, r))
+    const int32_t n = akv_held(p.tab, p.kv.bs_log2, r);
+    if (threadIdx.x == 0 && p.tab.lengths[r] > n)
       akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, r, p.tab.lengths[r], p.tab.width);
-    if (row_extent(p, r).chunks == 0) {
+    if (n == 0) {
       const int32_t heads = p.kv.heads * p.group;
       for (int64_t i = threadIdx.x; i < static_cast<int64_t>(heads) * dim; i += kThreads)
         finish<T>(p, r, static_cast<int32_t>(i / dim), static_cast<int>(i % dim), 0.f, 0.f);
@@ -613,144 +710,151 @@ __global__ void __launch_bounds__(kThreads, Eng::kCtas) k_attend(AttendParams p)
     const int32_t a = static_cast<int32_t>(rest - static_cast<int64_t>(pair) * e.chunks);
     const int32_t n = static_cast<int32_t>(end - x < e.chunks - a ? end - x : e.chunks - a);
     const int32_t h = pair / p.parts, part = pair % p.parts;
+    const bool whole = a == 0 && n == e.chunks;
+    const int cols = min(kC, p.group - part * kC);
+    const int32_t head0 = h * p.group + part * kC;
     {
       Eng eng;
       eng.run(p, e, s, h, part, e.first + a, e.first + a + n, warp, lane);
-      eng.store(acc + warp * kH * dim, ml[warp], dim, lane);
+      eng.store(acc + warp * kC * dim, ml[warp], dim, lane);
     }
     __syncthreads();
-    if (threadIdx.x < kH) {
-      const int i = threadIdx.x;
-      float top = -INFINITY, sum = 0.f;
+    if (threadIdx.x < kC) {
+      const int c = threadIdx.x;
+      float top = kLowest, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w][i].x);
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w][c].x);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        factor[w][i] = join_factor(ml[w][i].x, top);
-        sum += factor[w][i] * ml[w][i].y;
+        factor[w][c] = join_factor(ml[w][c], top);
+        sum += factor[w][c] * ml[w][c].y;
       }
-      joined[i] = make_float2(top, sum);
+      joined[c] = make_float2(top, sum);
     }
     __syncthreads();
-    const bool whole = a == 0 && n == e.chunks;
-    const int32_t left = p.group - part * kH;
-    const int heads = left < kH ? left : kH;
-    float* piece = nullptr;
-    if (!whole) {
-      // a pair that begins here and goes on is the CTA's second piece
-      piece = p.pieces + (blockIdx.x * 2ll + (a == 0 ? 1 : 0)) * piece_floats(kH, dim);
-      if (a == 0) {
-        const int64_t stop = x + e.chunks;
-        int64_t last = (stop * ctas + total - 1) / total - 1;
-        while (total * (last + 1) / ctas < stop) ++last;
-        while (last > blockIdx.x && total * last / ctas >= stop) --last;
-        meta = AttendMeta{s, h, part, static_cast<int32_t>(last - blockIdx.x)};
-      }
-    }
-    for (int i = threadIdx.x; i < heads * dim; i += kThreads) {
-      const int head = i / dim, d = i - head * dim;
+    // the CTAs of the pair; a CTA's first piece may go on from the CTA before
+    // it, its second begins in it
+    const int64_t c0 = whole ? blockIdx.x : deal.cta_of(x - a);
+    const int64_t c1 = whole ? blockIdx.x : deal.cta_of(x - a + e.chunks - 1);
+    const int64_t size = piece_floats(kC, dim);
+    auto slot = [&](int64_t c) { return p.pieces + (2 * c + (c == c0 ? 1 : 0)) * size; };
+    float* const mine = slot(blockIdx.x);
+    for (int i = threadIdx.x; i < cols * dim; i += kThreads) {
+      const int c = i / dim;
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w)
-        sum += factor[w][head] == 0.f ? 0.f : factor[w][head] * acc[(w * kH + head) * dim + d];
+        if (factor[w][c] != 0.f) sum = fmaf(factor[w][c], acc[w * kC * dim + i], sum);
       if (whole)
-        finish<T>(p, s, h * p.group + part * kH + head, d, sum, joined[head].y);
+        finish<T>(p, s, head0 + c, i - c * dim, sum, joined[c].y);
       else
-        piece[i] = sum;
+        mine[i] = sum;
     }
-    if (threadIdx.x < heads) {
-      const float2 j = joined[threadIdx.x];
-      if (whole)
-        finish_lse(p, s, h * p.group + part * kH + threadIdx.x, j.x, j.y);
+    auto finish_lses = [&]() {
+      if (threadIdx.x < cols) finish_lse(p, s, head0 + threadIdx.x, joined[threadIdx.x].x, joined[threadIdx.x].y);
+    };
+    auto keep_ml = [&](float* piece) {
+      if (threadIdx.x < cols) *reinterpret_cast<float2*>(piece + kC * dim + 2 * threadIdx.x) = joined[threadIdx.x];
+    };
+    // true in the CTA that is the last of `all` to come
+    auto last_of = [&](int32_t* counter, int64_t all) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        order = atomicAdd(counter, 1);
+        if (order == all - 1) *counter = 0;  // for the next launch
+      }
+      __syncthreads();
+      const bool last = order == all - 1;
+      if (last) __threadfence();
+      return last;
+    };
+    // Joins `all` pieces, piece i at piece(i): their sums go to put(c, d, sum).
+    auto join = [&](int all, auto piece, auto put) {
+      float2* const parts = reinterpret_cast<float2*>(acc);  // [all][cols]: (factor, l)
+      for (int i = threadIdx.x; i < all * cols; i += kThreads)
+        parts[i] = __ldcg(reinterpret_cast<const float2*>(piece(i / cols) + kC * dim) + i % cols);
+      __syncthreads();
+      if (threadIdx.x < cols) {
+        float2* const of = parts + threadIdx.x;
+        float top = kLowest, sum = 0.f;
+        for (int i = 0; i < all; ++i) top = fmaxf(top, of[i * cols].x);
+        for (int i = 0; i < all; ++i) {
+          const float f = join_factor(of[i * cols], top);
+          sum += f * of[i * cols].y;
+          of[i * cols].x = f;
+        }
+        joined[threadIdx.x] = make_float2(top, sum);
+      }
+      __syncthreads();
+      // 8 pieces' words at a time: they come from L2, one latency for all
+      auto sum_up = [&](auto word) {
+        using W = decltype(word);
+        constexpr int kE = sizeof(W) / 4;
+        for (int i = threadIdx.x * kE; i < cols * dim; i += kThreads * kE) {
+          const int c = i / dim;
+          float sum[kE] = {};
+          for (int k0 = 0; k0 < all; k0 += 8) {
+            W o[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = __ldcg(reinterpret_cast<const W*>(piece(min(k0 + k, all - 1)) + i));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float f = k0 + k < all ? parts[(k0 + k) * cols + c].x : 0.f;
+#pragma unroll
+              for (int j = 0; j < kE; ++j)
+                if (f != 0.f) sum[j] = fmaf(f, reinterpret_cast<const float*>(&o[k])[j], sum[j]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kE; ++j) put(c, i + j - c * dim, sum[j]);
+        }
+      };
+      if (dim % 4 == 0)
+        sum_up(float4{});
       else
-        *reinterpret_cast<float2*>(piece + kH * dim + 2 * threadIdx.x) = j;
+        sum_up(float{});
+    };
+    if (whole) {
+      finish_lses();
+    } else {
+      auto put = [&](int c, int d, float sum) { finish<T>(p, s, head0 + c, d, sum, joined[c].y); };
+      const int64_t first = c0 + (blockIdx.x - c0) / kFan * kFan;  // of this piece's sixteen
+      const int64_t near = min(static_cast<int64_t>(kFan), c1 + 1 - first), all = (c1 - c0) / kFan + 1;
+      keep_ml(mine);
+      if (last_of(p.arrived + 2 * first + (first == c0 ? 1 : 0), near)) {
+        auto piece = [&](int i) { return slot(first + i); };
+        if (all == 1) {
+          join(static_cast<int>(near), piece, put);
+          finish_lses();
+        } else {
+          float* const to = slot(first);
+          join(static_cast<int>(near), piece, [&](int c, int d, float sum) { to[c * dim + d] = sum; });
+          keep_ml(to);
+          if (last_of(p.arrived + 2ll * gridDim.x + c0, all)) {
+            join(static_cast<int>(all), [&](int i) { return slot(c0 + i * kFan); }, put);
+            finish_lses();
+          }
+        }
+      }
     }
     __syncthreads();
     x += n;
     rest += n;
-  }
-  if (!p.direct && threadIdx.x == 0) p.meta[blockIdx.x] = meta;
-}
-
-// Joins the pieces of the pair that began in CTA blockIdx.x and went on:
-// that CTA's second piece and the first pieces of the CTAs behind it.
-// `split` warps share a head's pieces, 8 / split heads per CTA.
-constexpr int kJoinThreads = 256;
-
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) k_join(AttendParams p, int32_t heads_per_pair, int32_t split) {
-  constexpr int kX = 8;  // dimensions per lane: head dims up to 256
-  __shared__ float sums[kJoinThreads / 32][kX * 32];
-  akv_grid_wait();
-  if (akv_failed(p.st)) return;
-  const AttendMeta meta = p.meta[blockIdx.x];
-  if (meta.pieces <= 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = p.kv.dim;
-  const int head = blockIdx.y * (kJoinThreads / 32 / split) + warp / split, sub = warp % split;
-  const int32_t left = p.group - meta.part * heads_per_pair;
-  const bool live = head < heads_per_pair && head < left;
-  const int64_t size = piece_floats(heads_per_pair, dim);
-  const int n = meta.pieces + 1;
-  auto slot = [&](int i) -> const float* {
-    return p.pieces + (i == 0 ? blockIdx.x * 2ll + 1 : (static_cast<int64_t>(blockIdx.x) + i) * 2) * size;
-  };
-  float m = -INFINITY, l = 0.f, o[kX];
-#pragma unroll
-  for (int x = 0; x < kX; ++x) o[x] = 0.f;
-  if (live) {
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, slot(i)[heads_per_pair * dim + 2 * head]);
-#pragma unroll
-    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullWarp, m, off));
-    for (int i = lane; i < n; i += 32) {
-      const float2 ml = *reinterpret_cast<const float2*>(slot(i) + heads_per_pair * dim + 2 * head);
-      l += join_factor(ml.x, m) * ml.y;
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(kFullWarp, l, off);
-#pragma unroll 2
-    for (int i = sub; i < n; i += split) {
-      const float* at = slot(i);
-      const float f = join_factor(at[heads_per_pair * dim + 2 * head], m);
-      if (f == 0.f) continue;
-#pragma unroll
-      for (int x = 0; x < kX; ++x) {
-        const int d = x * 32 + lane;
-        if (d < dim) o[x] = fmaf(f, at[head * dim + d], o[x]);
-      }
-    }
-  }
-  if (split > 1) {
-#pragma unroll
-    for (int x = 0; x < kX; ++x) sums[warp][x * 32 + lane] = o[x];
-    __syncthreads();
-    if (sub == 0)
-      for (int w = 1; w < split; ++w)
-#pragma unroll
-        for (int x = 0; x < kX; ++x) o[x] += sums[warp + w][x * 32 + lane];
-  }
-  if (live && sub == 0) {
-    const int32_t qh = meta.head * p.group + meta.part * heads_per_pair + head;
-#pragma unroll
-    for (int x = 0; x < kX; ++x) {
-      const int d = x * 32 + lane;
-      if (d < dim) finish<T>(p, meta.row, qh, d, o[x], l);
-    }
-    if (lane == 0) finish_lse(p, meta.row, qh, m, l);
   }
 }
 
 // ── host ───────────────────────────────────────────────────────────────────
 struct Kernel {
   void (*attend)(AttendParams) = nullptr;
-  void (*join)(AttendParams, int32_t, int32_t) = nullptr;
-  int heads = 0;  // query heads per pair
-  int ctas = 0;   // per SM
+  int cols = 0;  // query heads per pair
+  int ctas = 0;  // per SM
   const char* name = "";
 };
 
 template <class Eng>
 Kernel kernel_of(const char* name) {
-  return {k_attend<Eng>, k_join<typename Eng::Type>, Eng::kHeads, Eng::kCtas, name};
+  return {k_attend<Eng>, Eng::kCols, Eng::kCtas, name};
 }
 
 template <typename T>
@@ -767,15 +871,16 @@ Kernel mma_kernel(int dim, int group) {
 }
 
 // The widest word that the head dim and the addresses allow, at most 16
-// bytes and at most 4 elements.
+// bytes and at most 4 elements, and no more lanes than a row fills.
 template <typename T>
 Kernel simt_kernel(int dim, int group, int elements) {
   const bool wide = group > 2;
-  if (elements >= 4 && dim % 4 == 0 && dim > 64)
-    return wide ? kernel_of<SimtEngine<T, 4, 2, 8>>("simt 4x2x8") : kernel_of<SimtEngine<T, 4, 2, 2>>("simt 4x2x2");
-  if (elements >= 2 && dim % 2 == 0)
-    return wide ? kernel_of<SimtEngine<T, 2, 4, 8>>("simt 2x4x8") : kernel_of<SimtEngine<T, 2, 4, 2>>("simt 2x4x2");
-  return wide ? kernel_of<SimtEngine<T, 1, 8, 8>>("simt 1x8x8") : kernel_of<SimtEngine<T, 1, 8, 2>>("simt 1x8x2");
+  if (elements >= 4 && dim % 4 == 0) {
+    if (dim <= 64) return wide ? kernel_of<SimtEngine<T, 4, 1, 16, 8>>("simt 64x8") : kernel_of<SimtEngine<T, 4, 1, 16, 2>>("simt 64x2");
+    if (dim <= 128) return wide ? kernel_of<SimtEngine<T, 4, 1, 32, 8>>("simt 128x8") : kernel_of<SimtEngine<T, 4, 1, 32, 2>>("simt 128x2");
+    return wide ? kernel_of<SimtEngine<T, 4, 2, 32, 8>>("simt 256x8") : kernel_of<SimtEngine<T, 4, 2, 32, 2>>("simt 256x2");
+  }
+  return wide ? kernel_of<SimtEngine<T, 1, 8, 32, 8>>("simt 1x8") : kernel_of<SimtEngine<T, 1, 8, 32, 2>>("simt 1x2");
 }
 
 // `align`: the power of two that divides every address and stride, in bytes.
@@ -788,14 +893,14 @@ Kernel choose(int32_t dtype, int dim, int group, int align) {
   return dtype == AKV_F16 ? simt_kernel<__half>(dim, group, elements) : simt_kernel<__nv_bfloat16>(dim, group, elements);
 }
 
-constexpr int kDirectChunks = 4;  // tables of at most so many chunks: one CTA per pair, no joining launch
 constexpr int kMaxDim = 256;
 constexpr int64_t kMaxTokens = 1ll << 30;  // per row: positions are 32-bit numbers
 
+int parts_of(const Kernel& k, int group) { return akv_ceil_div(group, k.cols); }
 // Grid of a launch over `rows` rows of at most `chunks` chunks each.
-int64_t grid_of(const Kernel& k, int64_t rows, int64_t pairs, int64_t chunks, bool direct) {
-  if (direct) return rows * pairs;
+int64_t grid_of(const Kernel& k, int64_t rows, int64_t pairs, int64_t chunks) {
   const int64_t most = rows * pairs * chunks, fit = static_cast<int64_t>(kAkvSMs) * k.ctas;
+  static_assert(kAkvSMs * 3 <= kMaxCtas && 3 * kMaxCtas <= AKV_ATTENTION_COUNTERS, "two levels of joining");
   return most < 1 ? 1 : (most < fit ? most : fit);
 }
 
@@ -804,16 +909,12 @@ int64_t chunks_of(int32_t block_size, int32_t width, int32_t keep) {
   return (blocks * block_size + kChunk - 1) / kChunk;
 }
 
-int64_t scratch_of(const Kernel& k, int64_t grid, int dim) {
-  return grid * (2 * piece_floats(k.heads, dim) * 4 + static_cast<int64_t>(sizeof(AttendMeta)));
-}
+int64_t scratch_of(const Kernel& k, int64_t grid, int dim) { return grid * 2 * piece_floats(k.cols, dim) * 4; }
 
-// at most 32 KiB: 16 heads of 128 dimensions, or 8 of 256
-size_t shared_of(const Kernel& k, int dim) { return static_cast<size_t>(kWarps) * k.heads * dim * 4; }
-
-int prepare(const Kernel& k) {
-  if (int rc = akv_load_kernel(reinterpret_cast<const void*>(k.attend), k.name)) return rc;
-  return akv_load_kernel(reinterpret_cast<const void*>(k.join), k.name);
+// The warps' sums; joining takes their place for a (factor, l) per piece and column.
+size_t shared_of(const Kernel& k, int dim) {
+  const int sums = kWarps * k.cols * dim * 4, join = 2 * kFan * k.cols * 8;
+  return static_cast<size_t>(sums > join ? sums : join);  // at most 32 KiB
 }
 
 int power_of_two_in(uint64_t bits) {
@@ -860,13 +961,12 @@ int akv_tables_view(const char* what, const AkvPageBatch* b, int32_t block_size,
 
 int akv_attend_prepare() {
   for (int32_t dtype : {AKV_F32, AKV_F16, AKV_BF16})
-    for (int group : {1, 4, 9}) {
-      for (int dim : {64, 96, 128, 256})
-        if (int rc = prepare(choose(dtype, dim, group, 16))) return rc;
-      for (int align : {1, 2, 4, 8, 16})
-        if (align >= akv_dtype_bytes(dtype))
-          if (int rc = prepare(choose(dtype, 80, group, align))) return rc;
-    }
+    for (int group : {1, 4, 9})
+      for (int dim : {60, 64, 96, 100, 128, 200, 256})
+        for (int align : {4, 16}) {
+          const Kernel k = choose(dtype, dim, group, align);
+          if (int rc = akv_load_kernel(reinterpret_cast<const void*>(k.attend), k.name)) return rc;
+        }
   return AKV_OK;
 }
 
@@ -879,12 +979,12 @@ extern "C" int64_t akv_paged_attention_scratch_bytes(const AkvPagedPool* pool, i
     return -1;
   }
   const int64_t chunks = chunks_of(pool->block_size, table_width, keep);
-  if (rows == 0 || chunks <= kDirectChunks) return 0;
+  if (rows == 0) return 0;
   int64_t most = 0;
   for (int align : {4, 16}) {  // whichever engine the addresses will allow
     const Kernel k = choose(pool->dtype, kv.dim, group, align);
-    const int64_t pairs = static_cast<int64_t>(kv.heads) * akv_ceil_div(group, k.heads);
-    const int64_t n = scratch_of(k, grid_of(k, rows, pairs, chunks, false), kv.dim);
+    const int64_t pairs = static_cast<int64_t>(kv.heads) * parts_of(k, group);
+    const int64_t n = scratch_of(k, grid_of(k, rows, pairs, chunks), kv.dim);
     most = n > most ? n : most;
   }
   return most;
@@ -893,7 +993,7 @@ extern "C" int64_t akv_paged_attention_scratch_bytes(const AkvPagedPool* pool, i
 extern "C" int akv_paged_attention(const AkvPagedPool* pool, const AkvPageBatch* batch, const AkvHeads* query,
                                    int32_t group, float scale, int32_t window, const int32_t* selected, int32_t keep,
                                    const AkvHeads* out, float* lse, void* scratch, int64_t scratch_bytes,
-                                   AkvStatus* status, void* stream) {
+                                   int32_t* counters, AkvStatus* status, void* stream) {
   const char* what = "akv_paged_attention";
   AttendParams p;
   if (int rc = akv_layer_view(what, pool, &p.kv)) return rc;
@@ -908,7 +1008,7 @@ extern "C" int akv_paged_attention(const AkvPagedPool* pool, const AkvPageBatch*
                 "%s: negative stride", what);
   const int es = akv_dtype_bytes(pool->dtype);
   AKV_ARG_CHECK(akv_aligned(query->data, es) && akv_aligned(out->data, es) && akv_aligned(lse, 4) &&
-                    akv_aligned(scratch, 16),
+                    akv_aligned(scratch, 16) && akv_aligned(counters, 4),
                 "%s: misaligned pointer", what);
   const uint64_t bits = reinterpret_cast<uintptr_t>(pool->data) | reinterpret_cast<uintptr_t>(query->data) |
                         static_cast<uint64_t>(p.kv.row_bytes) | static_cast<uint64_t>(query->stride_token * es) |
@@ -924,37 +1024,19 @@ extern "C" int akv_paged_attention(const AkvPagedPool* pool, const AkvPageBatch*
   p.out_head = out->stride_head;
   p.lse = lse;
   p.group = group;
-  p.parts = akv_ceil_div(group, k.heads);
+  p.parts = parts_of(k, group);
   p.scale_log2 = scale * kLog2e;
   p.window = window;
   p.st = status;
-  const int64_t pairs = static_cast<int64_t>(p.kv.heads) * p.parts;
-  const int64_t chunks = chunks_of(pool->block_size, p.tab.width, p.keep);
-  p.direct = chunks <= kDirectChunks;
-  const int64_t grid = grid_of(k, p.tab.rows, pairs, chunks, p.direct);
-  AKV_ARG_CHECK(grid <= INT_MAX, "%s: too many rows", what);
-  const int64_t need = p.direct ? 0 : scratch_of(k, grid, p.kv.dim);
-  AKV_ARG_CHECK(scratch_bytes >= need && (scratch || need == 0), "%s: scratch has %lld bytes, %lld are needed", what,
+  const int64_t grid = grid_of(k, p.tab.rows, static_cast<int64_t>(p.kv.heads) * p.parts,
+                               chunks_of(pool->block_size, p.tab.width, p.keep));
+  const int64_t need = scratch_of(k, grid, p.kv.dim);
+  AKV_ARG_CHECK(scratch && scratch_bytes >= need, "%s: scratch has %lld bytes, %lld are needed", what,
                 static_cast<long long>(scratch_bytes), static_cast<long long>(need));
-  p.meta = static_cast<AttendMeta*>(scratch);
-  p.pieces = reinterpret_cast<float*>(p.meta + (p.direct ? 0 : grid));
-  cudaStream_t st = akv_stream(stream);
-  k.attend<<<static_cast<unsigned>(grid), kThreads, shared_of(k, p.kv.dim), st>>>(p);
+  AKV_ARG_CHECK(counters, "%s: NULL counters", what);
+  p.pieces = static_cast<float*>(scratch);
+  p.arrived = counters;
+  k.attend<<<static_cast<unsigned>(grid), kThreads, shared_of(k, p.kv.dim), akv_stream(stream)>>>(p);
   AKV_LAUNCH_CHECK(what);
-  if (p.direct) return AKV_OK;
-  // few pairs leave many pieces each: the more warps share a head's
-  const int32_t split = static_cast<int64_t>(p.tab.rows) * pairs * 8 <= grid ? 8 : 2;
-  const int32_t per = kJoinThreads / 32 / split;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid), akv_ceil_div(group < k.heads ? group : k.heads, per));
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, k.join, p, static_cast<int32_t>(k.heads), split);
-  if (err != cudaSuccess) return akv_cuda_fail(err, what);
   return AKV_OK;
 }

@@ -737,14 +737,19 @@ AKV_API int akv_key_bounds(const AkvPagedPool* pool, const AkvPageBatch* batch, 
  * of the sum of the scores' exponentials.
  *
  * scratch: akv_paged_attention_scratch_bytes() bytes of device memory, 16-byte
- * aligned, for this call alone until it has run; no initial contents.  An
- * id out of range is reported (AKV_ERR_OUT_OF_RANGE) and its positions left out. */
+ * aligned, for this call alone until it has run; no initial contents.
+ * counters: AKV_ATTENTION_COUNTERS int32 of device memory, zero before the
+ * first call and zero again when a call has run; calls that share them must
+ * not overlap on the GPU (one array per stream, one per captured call).  An id
+ * out of range is reported (AKV_ERR_OUT_OF_RANGE) and its positions left out;
+ * status is written only (an earlier error does not stop the call). */
+enum { AKV_ATTENTION_COUNTERS = 1536 };
 AKV_API int64_t akv_paged_attention_scratch_bytes(const AkvPagedPool* pool, int32_t rows, int32_t table_width,
                                           int32_t group, int32_t keep);
 AKV_API int akv_paged_attention(const AkvPagedPool* pool, const AkvPageBatch* batch, const AkvHeads* query,
                         int32_t group, float scale, int32_t window, const int32_t* selected, int32_t keep,
                         const AkvHeads* out, float* lse, void* scratch, int64_t scratch_bytes,
-                        AkvStatus* status, void* stream);
+                        int32_t* counters, AkvStatus* status, void* stream);
 
 /* The blocks of each row that matter most to its new token, by a bound on
  * their keys' scores: for row s, key head h and block j of n =
