@@ -249,7 +249,8 @@ SIGNATURES = {
     ),
 }
 
-_POOL, _BATCH, _HEADS = C.POINTER(AkvPagedPool), C.POINTER(AkvPageBatch), C.POINTER(AkvHeads)
+# const AkvPagedPool* / AkvPageBatch* / AkvHeads*, as packed bytes
+_POOL = _BATCH = _HEADS = C.c_char_p
 SIGNATURES.update({
     "akv_kv_append": (C.c_int, [_POOL, _BATCH, _HEADS, _HEADS, _I32, _P, _P, _I32, _I32, _I32, _HEADS, _HEADS, _I32, _P,
                                 _P, _P]),

@@ -32,7 +32,8 @@ refused.
 
 from __future__ import annotations
 
-import ctypes
+import struct
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -43,10 +44,14 @@ from .kernels import _as_device_i32, _require_cuda, _status_buffer, raise_for_st
 _DTYPES = {torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
 _GRAPH_STATUS: dict = {}
 _COUNTERS: dict = {}
-_byref = ctypes.byref
+# the C ABI's structs, packed (a tenth of a ctypes.Structure's time, on a path that is all latency)
+_POOL = struct.Struct("@Piiiiiiii").pack
+_BATCH = struct.Struct("@PPqii").pack
+_HEADS = struct.Struct("@Pqq").pack
+_capturing = torch.cuda.is_current_stream_capturing
 
 
-def _status(device: torch.device, status: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+def _status(device: torch.device, status: Optional[torch.Tensor], capturing: bool) -> Optional[torch.Tensor]:
     """The caller's status record or the default one.  A captured call uses a
     record of the device that an eager call made (a record made while capturing
     would be cleared by replays of that one graph only); before any, none."""
@@ -54,27 +59,28 @@ def _status(device: torch.device, status: Optional[torch.Tensor]) -> Optional[to
         if status.dtype != torch.int32 or status.device != device or status.numel() * 4 < N.STATUS_BYTES:
             raise ValueError("status must be an int32 tensor of 8 elements on the pool's device")
         return status
-    if torch.cuda.is_current_stream_capturing():
+    if capturing:
         return _GRAPH_STATUS.get(device.index)
     if device.index not in _GRAPH_STATUS:
         _GRAPH_STATUS[device.index] = torch.zeros(N.STATUS_BYTES // 4, dtype=torch.int32, device=device)
     return _status_buffer(device)
 
 
-def _counters(device: torch.device) -> torch.Tensor:
+def _counters(device: torch.device, stream: int, capturing: bool) -> torch.Tensor:
     """The arrival counters of paged_attention, zero between calls: one
     array per device and stream, and one of its own for a captured call, whose
     replays may overlap other work of any stream."""
-    if torch.cuda.is_current_stream_capturing():
+    if capturing:
         return torch.zeros(N.ATTENTION_COUNTERS, dtype=torch.int32, device=device)
-    key = (device.index, stream_handle(device))
+    key = (device.index, stream)
     buf = _COUNTERS.get(key)
     if buf is None:
         buf = _COUNTERS[key] = torch.zeros(N.ATTENTION_COUNTERS, dtype=torch.int32, device=device)
     return buf
 
 
-def _pool_view(pool: torch.Tensor, layer: int, what: str) -> N.AkvPagedPool:
+def _pool_view(pool: torch.Tensor, layer: int, what: str) -> bytes:
+    """AkvPagedPool of one layer."""
     shape = pool.shape
     if len(shape) != 6 or shape[2] != 2 or not pool.is_contiguous():
         raise ValueError(f"{what}: pool must be a contiguous "
@@ -82,39 +88,45 @@ def _pool_view(pool: torch.Tensor, layer: int, what: str) -> N.AkvPagedPool:
     dtype = _DTYPES.get(pool.dtype)
     if dtype is None:
         raise ValueError(f"{what}: pool dtype must be float16, bfloat16 or float32, got {pool.dtype}")
-    return N.AkvPagedPool(pool.data_ptr(), shape[0], shape[1], shape[3], shape[4], shape[5], dtype, int(layer), 0)
+    n, layers, _, heads, bs, dim = shape
+    return _POOL(pool.data_ptr(), n, layers, heads, bs, dim, dtype, layer, 0)
 
 
 def _batch_view(tables, lengths, device: torch.device, what: str):
-    """The batch's view, and the tensors it points into."""
+    """AkvPageBatch, its rows and width, and the tensors it points into."""
     if not (isinstance(tables, torch.Tensor) and tables.dtype == torch.int32 and tables.device == device):
         tables = _as_device_i32(tables, device)
     if not (isinstance(lengths, torch.Tensor) and lengths.dtype == torch.int32 and lengths.device == device):
         lengths = _as_device_i32(lengths, device)
-    if tables.dim() != 2 or lengths.dim() != 1 or tables.shape[0] != lengths.shape[0]:
+    shape = tables.shape
+    if len(shape) != 2 or lengths.dim() != 1 or shape[0] != lengths.shape[0]:
         raise ValueError(f"{what}: tables must be [rows, width] and lengths [rows], got {tuple(tables.shape)} "
                          f"and {tuple(lengths.shape)}")
-    if tables.stride(1) != 1 and tables.shape[1] > 1:
+    rows, width = shape
+    stride, step = tables.stride()
+    if step != 1 and width > 1:
         tables = tables.contiguous()
+        stride = width
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
-    rows, width = tables.shape
-    return N.AkvPageBatch(tables.data_ptr(), lengths.data_ptr(), tables.stride(0), width, rows), tables, lengths
+    return _BATCH(tables.data_ptr(), lengths.data_ptr(), stride, width, rows), rows, width, tables, lengths
 
 
-def _heads_view(x: torch.Tensor, pool: torch.Tensor, name: str, what: str) -> N.AkvHeads:
-    """View of a [tokens, heads, head_dim] operand of the pool's (or the
+def _heads_view(x: torch.Tensor, pool: torch.Tensor, name: str, what: str) -> bytes:
+    """AkvHeads of a [tokens, heads, head_dim] operand of the pool's (or the
     bounds') head_dim, type and device."""
-    if x.dim() != 3 or x.shape[2] != pool.shape[-1]:
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != pool.shape[-1]:
         raise ValueError(f"{what}: {name} must be [tokens, heads, {pool.shape[-1]}], got {tuple(x.shape)}")
     if x.dtype != pool.dtype or x.device != pool.device:
         raise ValueError(f"{what}: {name} must have the pool's dtype and device ({pool.dtype}, {pool.device}), "
                          f"got {x.dtype}, {x.device}")
-    if x.stride(2) != 1 and x.shape[2] > 1:
+    token, head, step = x.stride()
+    if step != 1 and shape[2] > 1:
         raise ValueError(f"{what}: {name}'s head_dim must be contiguous")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: {name} asks for a gradient; this is a forward-only operator")
-    return N.AkvHeads(x.data_ptr(), x.stride(0), x.stride(1))
+    return _HEADS(x.data_ptr(), token, head)
 
 
 def _query_heads(query: torch.Tensor, pool_heads: int, what: str) -> int:
@@ -159,10 +171,14 @@ def _check_bounds(bounds: torch.Tensor, pool: torch.Tensor, what: str) -> None:
                          f"got {tuple(bounds.shape)} {bounds.dtype} on {bounds.device}")
 
 
-def _scratch(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
-    if nbytes < 0:
+@lru_cache(maxsize=1024)
+def _attention_scratch(geometry: bytes, rows: int, width: int, group: int, keep: int) -> int:
+    """Work space of a call, a function of these numbers alone (`geometry`: an
+    AkvPagedPool without its address)."""
+    n = N.lib.akv_paged_attention_scratch_bytes(bytes(8) + geometry, rows, width, group, keep)
+    if n < 0:
         N.check(N.AKV_ERR_INVALID_ARG)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return n
 
 
 class _On:
@@ -172,7 +188,7 @@ class _On:
     __slots__ = ("guard",)
 
     def __init__(self, device: torch.device) -> None:
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+        self.guard = None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
     def __enter__(self) -> None:
         if self.guard is not None:
@@ -238,7 +254,7 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
         if query.shape[0] != tokens:
             raise ValueError(f"{what}: {query.shape[0]} queries for {tokens} keys")
         if query_out is None:
-            query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+            query_out = query.new_empty(query.shape)
         elif query_out is not query:
             same = query_out.data_ptr() == query.data_ptr() and query_out.stride() == query.stride()
             _check_output(query_out, query, "query_out", what, key, value, pool, *(() if same else (query,)))
@@ -251,30 +267,32 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
     if not _require_cuda(pool, what):
         return query_out
     dev = pool.device
-    b, tables, lengths = _batch_view(tables, lengths, dev, what)
+    b, rows, _, tables, lengths = _batch_view(tables, lengths, dev, what)
     sptr = None
     if starts is not None:
         if not (isinstance(starts, torch.Tensor) and starts.dtype == torch.int32 and starts.device == dev
                 and starts.is_contiguous()):
             starts = _as_device_i32(starts, dev)
-        if starts.shape != (b.rows + 1,):
-            raise ValueError(f"{what}: starts must be [{b.rows + 1}], got {tuple(starts.shape)}")
+        if starts.shape != (rows + 1,):
+            raise ValueError(f"{what}: starts must be [{rows + 1}], got {tuple(starts.shape)}")
         sptr = starts.data_ptr()
     rptr, positions, rotary = None, 0, 0
     if rope is not None:
         if rope.dim() != 2 or rope.dtype != torch.float32 or rope.device != dev or not rope.is_contiguous():
             raise ValueError(f"{what}: rope must be a contiguous float32 [positions, rotary_dim] tensor on {dev}")
+        if rope.data_ptr() % 16:
+            raise ValueError(f"{what}: rope must start on a 16-byte boundary")
         rptr, (positions, rotary) = rope.data_ptr(), rope.shape
     bptr = None
     if bounds is not None:
         _check_bounds(bounds, pool, what)
         bptr = bounds.data_ptr()
     with _On(dev):
-        st = _status(dev, status)
-        N.check(N.lib.akv_kv_append(
-            _byref(p), _byref(b), _byref(kview), _byref(vview), tokens, sptr, rptr, positions, rotary, int(interleaved),
-            None if qview is None else _byref(qview), None if oview is None else _byref(oview), heads, bptr,
-            None if st is None else st.data_ptr(), stream_handle(dev)))
+        st = _status(dev, status, _capturing())
+        rc = N.lib.akv_kv_append(p, b, kview, vview, tokens, sptr, rptr, positions, rotary, interleaved, qview, oview,
+                                 heads, bptr, None if st is None else st.data_ptr(), stream_handle(dev))
+        if rc:
+            N.check(rc)
         if check and st is not None:
             raise_for_status(st)
     return query_out
@@ -298,10 +316,10 @@ def key_bounds(pool: torch.Tensor, layer: int, tables, lengths, bounds: Optional
     if not _require_cuda(pool, what):
         return bounds
     dev = pool.device
-    b, tables, lengths = _batch_view(tables, lengths, dev, what)
+    b, _, _, tables, lengths = _batch_view(tables, lengths, dev, what)
     with _On(dev):
-        st = _status(dev, status)
-        N.check(N.lib.akv_key_bounds(_byref(p), _byref(b), bounds.data_ptr(), None if st is None else st.data_ptr(),
+        st = _status(dev, status, _capturing())
+        N.check(N.lib.akv_key_bounds(p, b, bounds.data_ptr(), None if st is None else st.data_ptr(),
                                      stream_handle(dev)))
         if check and st is not None:
             raise_for_status(st)
@@ -333,21 +351,23 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, layer: int, tables,
     group = _query_heads(query, H, what)
     qview = _heads_view(query, bounds, "query", what)
     rows = query.shape[0]
-    selected = torch.empty((rows, H, keep), dtype=torch.int32, device=query.device)
+    selected = query.new_empty((rows, H, keep), dtype=torch.int32)
     if not _require_cuda(bounds, what):
         return selected
     dev = bounds.device
-    p = N.AkvPagedPool(None, n, L, H, int(block_size), D, dtype, int(layer), 0)
-    b, tables, lengths = _batch_view(tables, lengths, dev, what)
-    if b.rows != rows:
-        raise ValueError(f"{what}: {rows} queries for {b.rows} rows")
+    p = _POOL(0, n, L, H, block_size, D, dtype, layer, 0)
+    b, batch, width, tables, lengths = _batch_view(tables, lengths, dev, what)
+    if batch != rows:
+        raise ValueError(f"{what}: {rows} queries for {batch} rows")
     with _On(dev):
-        st = _status(dev, status)
-        scratch = _scratch(N.lib.akv_select_blocks_scratch_bytes(rows, H, b.table_width, keep), dev)
-        N.check(N.lib.akv_select_blocks(
-            _byref(p), bounds.data_ptr(), _byref(b), _byref(qview), group, keep, first, last, selected.data_ptr(),
-            None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(),
-            None if st is None else st.data_ptr(), stream_handle(dev)))
+        st = _status(dev, status, _capturing())
+        scratch = query.new_empty(max(0, N.lib.akv_select_blocks_scratch_bytes(rows, H, width, keep)),
+                                  dtype=torch.uint8)
+        rc = N.lib.akv_select_blocks(p, bounds.data_ptr(), b, qview, group, keep, first, last, selected.data_ptr(),
+                                     scratch.data_ptr(), scratch.numel(), None if st is None else st.data_ptr(),
+                                     stream_handle(dev))
+        if rc:
+            N.check(rc)
         if check and st is not None:
             raise_for_status(st)
     return selected
@@ -377,21 +397,21 @@ def paged_attention(query: torch.Tensor, pool: torch.Tensor, layer: int, tables,
     qview = _heads_view(query, pool, "query", what)
     rows, heads, dim = query.shape
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=query.dtype, device=query.device)
-        oview = N.AkvHeads(out.data_ptr(), heads * dim, dim)
+        out = query.new_empty((rows, heads, dim))
+        oview = _HEADS(out.data_ptr(), heads * dim, dim)
     else:
         _check_output(out, query, "out", what, query, pool)
         oview = _heads_view(out, pool, "out", what)
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=query.device) if return_lse else None
+    lse = query.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
     if not _require_cuda(pool, what):
         return (out, lse) if return_lse else out
     dev = pool.device
     window = int(window)
     if window < 0:
         raise ValueError(f"{what}: window must not be negative, got {window}")
-    b, tables, lengths = _batch_view(tables, lengths, dev, what)
-    if b.rows != rows:
-        raise ValueError(f"{what}: {rows} queries for {b.rows} rows")
+    b, batch, width, tables, lengths = _batch_view(tables, lengths, dev, what)
+    if batch != rows:
+        raise ValueError(f"{what}: {rows} queries for {batch} rows")
     sel, keep = None, 0
     if selected is not None:
         keep = selected.shape[-1] if selected.dim() == 3 else 0
@@ -401,14 +421,15 @@ def paged_attention(query: torch.Tensor, pool: torch.Tensor, layer: int, tables,
                              f"on {dev}")
         sel = selected.data_ptr()
     with _On(dev):
-        st = _status(dev, status)
-        scratch = _scratch(N.lib.akv_paged_attention_scratch_bytes(_byref(p), rows, b.table_width, group, keep), dev)
-        counters = _counters(dev)
-        N.check(N.lib.akv_paged_attention(
-            _byref(p), _byref(b), _byref(qview), group, dim ** -0.5 if scale is None else scale,
-            min(window, (1 << 31) - 1), sel, keep, _byref(oview), None if lse is None else lse.data_ptr(),
-            None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(),
-            counters.data_ptr(), None if st is None else st.data_ptr(), stream_handle(dev)))
+        capturing = _capturing()
+        st, stream = _status(dev, status, capturing), stream_handle(dev)
+        scratch = query.new_empty(_attention_scratch(p[8:], rows, width, group, keep), dtype=torch.uint8)
+        rc = N.lib.akv_paged_attention(
+            p, b, qview, group, dim ** -0.5 if scale is None else scale, min(window, (1 << 31) - 1), sel, keep, oview,
+            None if lse is None else lse.data_ptr(), scratch.data_ptr(), scratch.numel(),
+            _counters(dev, stream, capturing).data_ptr(), None if st is None else st.data_ptr(), stream)
+        if rc:
+            N.check(rc)
         if check and st is not None:
             raise_for_status(st)
     return (out, lse) if return_lse else out

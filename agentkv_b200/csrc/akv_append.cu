@@ -11,10 +11,9 @@
 // for a decode step's few rows the launch and two dependent loads.
 //
 // Work: one unit per (row, block) that gets tokens, dealt to one or several
-// CTAs by heads; a thread takes one word (of kV elements, and the word of
-// their partners) of a head through the unit's tokens, so that a key's
-// bounds are that thread's own minimum and maximum: no atomics, and
-// the same result in any order.
+// CTAs by words of kV elements (with the word of their partners); the four
+// lanes that hold a key's word bring its bounds together: no atomics, and the
+// same result in any order.
 #include <climits>
 
 #include "akv_paged.cuh"
@@ -22,6 +21,9 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kHeads = 4;  // query heads that a thread turns together
+
+AKV_DEV int32_t akv_ceil_div_dev(int32_t a, int32_t b) { return (a + b - 1) / b; }
 
 struct AppendParams {
   AkvLayer kv;
@@ -92,51 +94,87 @@ struct Lane {
 };
 
 template <typename T, int kV>
+AKV_DEV AkvPack<T, kV> word_at(const char* row, int d) {
+  return akv_load<T, kV>(row + d * sizeof(T));
+}
+template <typename T, int kV>
 AKV_DEV void load_word(float (&x)[kV], const char* row, int d) {
-  const AkvVec<T, kV> w = *reinterpret_cast<const AkvVec<T, kV>*>(row + d * sizeof(T));
-#pragma unroll
-  for (int i = 0; i < kV; ++i) x[i] = to_f32<T>(w.v[i]);
+  akv_unpack<T, kV>(x, word_at<T, kV>(row, d));
 }
 
 // Rounds x to T (x holds the rounded values afterwards) and stores it.
 template <typename T, int kV>
 AKV_DEV void store_word(float (&x)[kV], char* row, int d) {
-  AkvVec<T, kV> w;
-#pragma unroll
-  for (int i = 0; i < kV; ++i) {
-    w.v[i] = from_f32<T>(x[i]);
-    x[i] = to_f32<T>(w.v[i]);
-  }
-  *reinterpret_cast<AkvVec<T, kV>*>(row + d * sizeof(T)) = w;
+  *reinterpret_cast<AkvPack<T, kV>*>(row + d * sizeof(T)) = akv_pack<T, kV>(x);
 }
 
-// x, y: the word(s) of one token at `pos`.
+// The cosines and sines of a word's pairs at one position.
+template <int kV>
+struct Turn {
+  float cos[kV], sin[kV];  // kV / 2 of each where the word holds whole pairs
+};
+
 template <typename T, int kV>
-AKV_DEV void rotate(const AppendParams& p, const Lane<T, kV>& ln, int32_t pos, float (&x)[kV], float (&y)[kV]) {
-  if (ln.pair < 0) return;
-  const float* cos_row = p.rope + static_cast<int64_t>(pos) * p.rotary;
+AKV_DEV Turn<kV> load_turn(const AppendParams& p, const Lane<T, kV>& ln, int32_t pos) {
+  Turn<kV> t = {};
+  if (ln.pair < 0) return t;
+  const float* cos_row = p.rope + static_cast<int64_t>(pos) * p.rotary + ln.pair;
   const float* sin_row = cos_row + p.rotary / 2;
+  // (words divide the rotary dimensions: their places in the table are as aligned)
+  constexpr int kStep = kV >= 8 ? 4 : kV, kHalf = kV > 1 ? kV / 2 : 1;
+  if (ln.b >= 0) {
+#pragma unroll
+    for (int i = 0; i < kV; i += kStep) {
+      float c[kStep], n[kStep];
+      akv_unpack<float, kStep>(c, akv_load<float, kStep>(cos_row + i));
+      akv_unpack<float, kStep>(n, akv_load<float, kStep>(sin_row + i));
+#pragma unroll
+      for (int j = 0; j < kStep; ++j) {
+        t.cos[i + j] = c[j];
+        t.sin[i + j] = n[j];
+      }
+    }
+  } else if (kV > 1) {
+    float c[kHalf], n[kHalf];
+    akv_unpack<float, kHalf>(c, akv_load<float, kHalf>(cos_row));
+    akv_unpack<float, kHalf>(n, akv_load<float, kHalf>(sin_row));
+#pragma unroll
+    for (int j = 0; j < kHalf; ++j) {
+      t.cos[j] = c[j];
+      t.sin[j] = n[j];
+    }
+  }
+  return t;
+}
+
+// Turns the word(s) x, y of one token.
+template <typename T, int kV>
+AKV_DEV void turn(const Turn<kV>& t, const Lane<T, kV>& ln, float (&x)[kV], float (&y)[kV]) {
+  if (ln.pair < 0) return;
   if (ln.b >= 0) {
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
-      const float c = cos_row[ln.pair + i], s = sin_row[ln.pair + i];
       const float u = x[i], v = y[i];
-      x[i] = u * c - v * s;
-      y[i] = v * c + u * s;
+      x[i] = u * t.cos[i] - v * t.sin[i];
+      y[i] = v * t.cos[i] + u * t.sin[i];
     }
-  } else if (kV > 1) {  // interleaved: kV / 2 whole pairs
+  } else if (kV > 1) {
 #pragma unroll
     for (int i = 0; i < kV / 2; ++i) {
-      const float c = cos_row[ln.pair + i], s = sin_row[ln.pair + i];
       const float u = x[2 * i], v = x[(2 * i + 1) % kV];
-      x[2 * i] = u * c - v * s;
-      x[(2 * i + 1) % kV] = v * c + u * s;
+      x[2 * i] = u * t.cos[i] - v * t.sin[i];
+      x[(2 * i + 1) % kV] = v * t.cos[i] + u * t.sin[i];
     }
   }
 }
 
 template <typename T, int kV>
-__global__ void __launch_bounds__(kThreads) k_append(AppendParams p) {
+AKV_DEV void rotate(const AppendParams& p, const Lane<T, kV>& ln, int32_t pos, float (&x)[kV], float (&y)[kV]) {
+  turn(load_turn(p, ln, pos), ln, x, y);
+}
+
+template <typename T, int kV>
+__global__ void __launch_bounds__(kThreads, 2) k_append(AppendParams p) {
   using Search = AkvRowSearch<kThreads>;
   __shared__ typename Search::Shared sh;
   if (akv_failed(p.st)) return;
@@ -182,12 +220,17 @@ __global__ void __launch_bounds__(kThreads) k_append(AppendParams p) {
   const int all = p.kv.dim / kV;
   const int words = partners(p, kV) ? all - p.rotary / 2 / kV : all;
   const int32_t heads = p.kv.heads;
-  const int64_t items = static_cast<int64_t>(heads) * (words + all) + static_cast<int64_t>(p.q_heads) * words;
+  // Items: a word of a key through every fourth token, four lanes next to one
+  // another for the four (they bring its bounds together); a word of a value,
+  // likewise; a word of one token of four query heads, which turn alike.
+  const int64_t keys = 4ll * heads * words, values = 4ll * heads * all;
+  const int64_t items = keys + values + static_cast<int64_t>(akv_ceil_div_dev(p.q_heads, kHeads)) * count * words;
   for (int64_t it = blockIdx.y * kThreads + threadIdx.x; it < items; it += static_cast<int64_t>(gridDim.y) * kThreads) {
-    if (it < static_cast<int64_t>(heads) * words) {  // a key
-      const int32_t h = static_cast<int32_t>(it / words);
+    if (it < keys) {
+      const int q = static_cast<int>(it & 3);
+      const int32_t h = static_cast<int32_t>((it >> 2) / words);
       Lane<T, kV> ln;
-      ln.set(p, static_cast<int>(it % words));
+      ln.set(p, static_cast<int>((it >> 2) % words));
       char* tile = page + h * p.kv.tile_bytes;
       float lo[kV], hi[kV], lo2[kV], hi2[kV];
 #pragma unroll
@@ -206,14 +249,14 @@ __global__ void __launch_bounds__(kThreads) k_append(AppendParams p) {
       };
       if (p.bounds)
 #pragma unroll 4
-        for (int32_t r = 0; r < in0; ++r) {
+        for (int32_t r = q; r < in0; r += 4) {
           float x[kV], y[kV] = {};
           load_word<T, kV>(x, tile + r * p.kv.row_bytes, ln.a);
           if (ln.b >= 0) load_word<T, kV>(y, tile + r * p.kv.row_bytes, ln.b);
           take(x, y);
         }
 #pragma unroll 4
-      for (int32_t t = 0; t < count; ++t) {
+      for (int32_t t = q; t < count; t += 4) {
         const char* src = p.key + (row0 + t) * p.k_tok + h * p.k_head;
         char* dst = tile + static_cast<int64_t>(in0 + t) * p.kv.row_bytes;
         float x[kV], y[kV] = {};
@@ -225,40 +268,60 @@ __global__ void __launch_bounds__(kThreads) k_append(AppendParams p) {
         take(x, y);
       }
       if (p.bounds) {
+        const uint32_t four = 0xfu << (threadIdx.x & 28);
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1)
+#pragma unroll
+          for (int i = 0; i < kV; ++i) {
+            lo[i] = min_nan(lo[i], __shfl_xor_sync(four, lo[i], off));
+            hi[i] = max_nan(hi[i], __shfl_xor_sync(four, hi[i], off));
+            lo2[i] = min_nan(lo2[i], __shfl_xor_sync(four, lo2[i], off));
+            hi2[i] = max_nan(hi2[i], __shfl_xor_sync(four, hi2[i], off));
+          }
         char* b = p.bounds + id * p.bounds_page + p.bounds_layer + static_cast<int64_t>(h) * 2 * p.kv.row_bytes;
-        store_word<T, kV>(lo, b, ln.a);
-        store_word<T, kV>(hi, b + p.kv.row_bytes, ln.a);
+        if (q == 0) store_word<T, kV>(lo, b, ln.a);
+        if (q == 1) store_word<T, kV>(hi, b + p.kv.row_bytes, ln.a);
         if (ln.b >= 0) {
-          store_word<T, kV>(lo2, b, ln.b);
-          store_word<T, kV>(hi2, b + p.kv.row_bytes, ln.b);
+          if (q == 2) store_word<T, kV>(lo2, b, ln.b);
+          if (q == 3) store_word<T, kV>(hi2, b + p.kv.row_bytes, ln.b);
         }
       }
-    } else if (it < static_cast<int64_t>(heads) * (words + all)) {  // a value: bits only
-      const int64_t i = it - static_cast<int64_t>(heads) * words;
-      const int32_t h = static_cast<int32_t>(i / all);
-      const int d = static_cast<int>(i % all) * kV * static_cast<int>(sizeof(T));
+    } else if (it < keys + values) {  // a value: bits only
+      const int64_t i = (it - keys) / all;
+      const int q = static_cast<int>(i & 3);
+      const int32_t h = static_cast<int32_t>(i >> 2);
+      const int d = static_cast<int>((it - keys) % all) * kV * static_cast<int>(sizeof(T));
       const char* src = p.value + row0 * p.v_tok + h * p.v_head + d;
       char* dst = page + p.kv.kv_bytes + h * p.kv.tile_bytes + static_cast<int64_t>(in0) * p.kv.row_bytes + d;
 #pragma unroll 4
-      for (int32_t t = 0; t < count; ++t)
-        *reinterpret_cast<AkvVec<T, kV>*>(dst + static_cast<int64_t>(t) * p.kv.row_bytes) =
-            *reinterpret_cast<const AkvVec<T, kV>*>(src + t * p.v_tok);
-    } else {  // a query
-      const int64_t i = it - static_cast<int64_t>(heads) * (words + all);
-      const int32_t h = static_cast<int32_t>(i / words);
+      for (int32_t t = q; t < count; t += 4)
+        *reinterpret_cast<AkvPack<T, kV>*>(dst + static_cast<int64_t>(t) * p.kv.row_bytes) =
+            akv_load<T, kV>(src + t * p.v_tok);
+    } else {  // queries
+      const int64_t i = (it - keys - values) / words;
+      const int32_t t = static_cast<int32_t>(i % count), h0 = static_cast<int32_t>(i / count) * kHeads;
       Lane<T, kV> ln;
-      ln.set(p, static_cast<int>(i % words));
-#pragma unroll 4
-      for (int32_t t = 0; t < count; ++t) {
-        const char* src = p.query + (row0 + t) * p.q_tok + h * p.q_head;
-        char* dst = p.query_out + (row0 + t) * p.o_tok + h * p.o_head;
-        float x[kV], y[kV] = {};
-        load_word<T, kV>(x, src, ln.a);
-        if (ln.b >= 0) load_word<T, kV>(y, src, ln.b);
-        rotate<T, kV>(p, ln, p0 + t, x, y);
-        store_word<T, kV>(x, dst, ln.a);
-        if (ln.b >= 0) store_word<T, kV>(y, dst, ln.b);
-      }
+      ln.set(p, static_cast<int>((it - keys - values) % words));
+      const Turn<kV> by = load_turn(p, ln, p0 + t);
+      const char* src = p.query + (row0 + t) * p.q_tok + h0 * p.q_head;
+      char* dst = p.query_out + (row0 + t) * p.o_tok + h0 * p.o_head;
+      AkvPack<T, kV> a[kHeads], b[kHeads];
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k)
+        if (h0 + k < p.q_heads) {
+          a[k] = word_at<T, kV>(src + k * p.q_head, ln.a);
+          if (ln.b >= 0) b[k] = word_at<T, kV>(src + k * p.q_head, ln.b);
+        }
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k)
+        if (h0 + k < p.q_heads) {
+          float x[kV], y[kV] = {};
+          akv_unpack<T, kV>(x, a[k]);
+          if (ln.b >= 0) akv_unpack<T, kV>(y, b[k]);
+          turn(by, ln, x, y);
+          store_word<T, kV>(x, dst + k * p.o_head, ln.a);
+          if (ln.b >= 0) store_word<T, kV>(y, dst + k * p.o_head, ln.b);
+        }
     }
   }
 }
@@ -307,7 +370,8 @@ using AppendKernel = void (*)(AppendParams);
 // the rotary half allow.
 template <typename T>
 AppendKernel append_kernel(int elements) {
-  if (elements >= 8 && sizeof(T) == 2) return k_append<T, 8>;
+  if constexpr (sizeof(T) == 2)
+    if (elements >= 8) return k_append<T, 8>;
   if (elements >= 4) return k_append<T, 4>;
   if (elements >= 2) return k_append<T, 2>;
   return k_append<T, 1>;
@@ -364,7 +428,7 @@ extern "C" int akv_kv_append(const AkvPagedPool* pool, const AkvPageBatch* batch
     bits |= reinterpret_cast<uintptr_t>(x->data) | static_cast<uint64_t>(x->stride_token * es) |
             static_cast<uint64_t>(x->stride_head * es);
   }
-  AKV_ARG_CHECK(akv_aligned(rope, 4) && akv_aligned(bounds, es), "%s: misaligned pointer", what);
+  AKV_ARG_CHECK(akv_aligned(rope, 16) && akv_aligned(bounds, es), "%s: misaligned pointer", what);
   // a word lies wholly in one half of the rotated pairs, or holds whole pairs
   if (rope) bits |= static_cast<uint64_t>(interleaved ? rotary_dim : rotary_dim / 2) * es;
   const int low = lowest_bit(bits);
@@ -399,7 +463,7 @@ extern "C" int akv_kv_append(const AkvPagedPool* pool, const AkvPageBatch* batch
   const int64_t units = starts == nullptr ? p.tab.rows : most < n_tokens ? most : n_tokens;
   // as many CTAs per unit as its words fill, while there are SMs for them
   const int64_t words = p.kv.dim / elements;
-  const int64_t items = words * (2ll * p.kv.heads + p.q_heads);
+  const int64_t items = words * (8ll * p.kv.heads + (starts ? 4ll : 1ll) * p.q_heads / kHeads);
   int64_t per = (items + kThreads - 1) / kThreads;
   const int64_t room = (8ll * kAkvSMs + units - 1) / units;
   per = per < room ? per : room;

@@ -38,6 +38,7 @@ constexpr float kLowest = -3.402823466e38f;
 // sums are the same for any m, so long as 2^(x - m) stays in range: at most
 // 2^8 here), which spares most steps the reduction over the lanes.
 constexpr float kLazy = 8.0f;
+constexpr int kLeast = 2;                  // chunks per CTA: a piece costs as much as one or two
 constexpr int kFan = 16;                   // pieces that are joined at a time
 constexpr int kMaxCtas = kFan * kFan * 2;  // two levels of joining
 
@@ -464,27 +465,21 @@ struct SimtEngine {
   static constexpr int kStep = kL / kVals;                // each held by this many lanes
   static constexpr int kPass = kU * kSub;                 // positions of a pass
   static_assert(kTile % kPass == 0 && kStep >= 1, "a tile is whole passes");
-  using Vec = AkvVec<T, kE>;
+  using Word = AkvPack<T, kE>;
 
   float q[kH][kX], o[kH][kX];
   float m, l;  // of this lane's head, l over this lane's positions
 
-  AKV_DEV static Vec zero() {
-    Vec w;
-#pragma unroll
-    for (int i = 0; i < kE; ++i) w.v[i] = from_f32<T>(0.f);
-    return w;
-  }
-  AKV_DEV static void load_row(Vec (&x)[kJ], const char* row, int dim, bool ok, int at) {
+  AKV_DEV static void load_row(Word (&x)[kJ], const char* row, int dim, bool ok, int at) {
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
       const int d = (j * kL + at) * kE;
-      x[j] = ok && d < dim ? *reinterpret_cast<const Vec*>(row + d * sizeof(T)) : zero();
+      x[j] = ok && d < dim ? akv_load<T, kE>(row + d * sizeof(T)) : Word{};
     }
   }
 
   AKV_DEV void load_pass(const AttendParams& p, const Cursor& cur, const char* kbase, int32_t chunk, uint32_t vm,
-                         int r0, int lane, Vec (&k)[kU][kJ], Vec (&v)[kU][kJ]) {
+                         int r0, int lane, Word (&k)[kU][kJ], Word (&v)[kU][kJ]) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int r = r0 + u * kSub + lane / kL;
@@ -494,8 +489,8 @@ struct SimtEngine {
     }
   }
 
-  AKV_DEV void compute(const AttendParams& p, uint32_t vm, int r0, int lane, const Vec (&k)[kU][kJ],
-                       const Vec (&v)[kU][kJ]) {
+  AKV_DEV void compute(const AttendParams& p, uint32_t vm, int r0, int lane, const Word (&k)[kU][kJ],
+                       const Word (&v)[kU][kJ]) {
     const int at = lane % kL, mine = at / kStep % kU;  // this lane's position of the kU
     float val[kVals];
 #pragma unroll
@@ -504,9 +499,12 @@ struct SimtEngine {
       for (int u = 0; u < kU; ++u) {
         float d = 0.f;
 #pragma unroll
-        for (int j = 0; j < kJ; ++j)
+        for (int j = 0; j < kJ; ++j) {
+          float x[kE];
+          akv_unpack<T, kE>(x, k[u][j]);
 #pragma unroll
-          for (int i = 0; i < kE; ++i) d = fmaf(q[n][j * kE + i], to_f32<T>(k[u][j].v[i]), d);
+          for (int i = 0; i < kE; ++i) d = fmaf(q[n][j * kE + i], x[i], d);
+        }
         val[n * kU + u] = d;
       }
     // value i ends, whole, in lanes i * kStep ..: each exchange keeps the
@@ -550,9 +548,12 @@ struct SimtEngine {
       for (int u = 0; u < kU; ++u) {
         const float f = __shfl_sync(kFullWarp, w, (lane & ~(kL - 1)) + (n * kU + u) * kStep);
 #pragma unroll
-        for (int j = 0; j < kJ; ++j)
+        for (int j = 0; j < kJ; ++j) {
+          float x[kE];
+          akv_unpack<T, kE>(x, v[u][j]);
 #pragma unroll
-          for (int i = 0; i < kE; ++i) o[n][j * kE + i] = fmaf(f, to_f32<T>(v[u][j].v[i]), o[n][j * kE + i]);
+          for (int i = 0; i < kE; ++i) o[n][j * kE + i] = fmaf(f, x[i], o[n][j * kE + i]);
+        }
       }
   }
 
@@ -563,12 +564,15 @@ struct SimtEngine {
     for (int n = 0; n < kH; ++n) {
       const int32_t head = part * kH + n;
       const T* row = static_cast<const T*>(p.q) + s * p.q_row + (static_cast<int64_t>(h) * p.group + head) * p.q_head;
-      Vec w[kJ];
+      Word w[kJ];
       load_row(w, reinterpret_cast<const char*>(row), p.kv.dim, head < p.group, lane % kL);
 #pragma unroll
-      for (int j = 0; j < kJ; ++j)
+      for (int j = 0; j < kJ; ++j) {
+        float x[kE];
+        akv_unpack<T, kE>(x, w[j]);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) q[n][j * kE + i] = to_f32<T>(w[j].v[i]);
+        for (int i = 0; i < kE; ++i) q[n][j * kE + i] = x[i];
+      }
 #pragma unroll
       for (int x = 0; x < kX; ++x) o[n][x] = 0.f;
     }
@@ -578,12 +582,12 @@ struct SimtEngine {
     Cursor cur;
     cur.refill(p, e, s, h, a, b, warp, lane);
     uint32_t vm = cur.valid(p, a, lane);
-    Vec k[kU][kJ], v[kU][kJ];
+    Word k[kU][kJ], v[kU][kJ];
     load_pass(p, cur, kbase, a, vm, 0, lane, k, v);
     for (int32_t chunk = a; chunk < b; ++chunk) {
 #pragma unroll 1
       for (int r0 = 0; r0 < kTile; r0 += kPass) {
-        Vec kn[kU][kJ], vn[kU][kJ];
+        Word kn[kU][kJ], vn[kU][kJ];
         const uint32_t now = vm;
         const bool last = r0 + kPass >= kTile, more = !last || chunk + 1 < b;
         if (last && more) {
@@ -680,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, Eng::kCtas) k_attend(AttendParams p)
     Search search;
     search.scan(sh, p.tab.rows, units);
     deal.total = search.total;
-    deal.ctas = gridDim.x < deal.total ? gridDim.x : deal.total;
+    deal.ctas = min(static_cast<int64_t>(gridDim.x), (deal.total + kLeast - 1) / kLeast);
     if (blockIdx.x < deal.ctas) {
       x = deal.begin(blockIdx.x);
       end = deal.begin(blockIdx.x + 1);

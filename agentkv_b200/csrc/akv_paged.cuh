@@ -3,6 +3,9 @@
 // batch, and programmatic dependent launch.
 #pragma once
 
+#include <cstring>
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -28,11 +31,65 @@ AKV_DEV __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <>
 AKV_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// `N` elements of T as one aligned word.
+template <int kBytes>
+struct AkvWord;
+template <>
+struct AkvWord<16> { using Type = uint4; };
+template <>
+struct AkvWord<8> { using Type = uint2; };
+template <>
+struct AkvWord<4> { using Type = uint32_t; };
+template <>
+struct AkvWord<2> { using Type = uint16_t; };
+
+// `N` elements of T as one word: loaded, held and stored whole (an array of
+// 16-bit elements takes a register each), taken apart where they are used.
 template <typename T, int N>
-struct alignas(sizeof(T) * N) AkvVec {
-  T v[N];
-};
+using AkvPack = typename AkvWord<static_cast<int>(sizeof(T)) * N>::Type;
+
+template <typename T, int N>
+AKV_DEV AkvPack<T, N> akv_load(const void* p) {
+  return *static_cast<const AkvPack<T, N>*>(p);
+}
+
+template <typename T, int N>
+AKV_DEV void akv_unpack(float (&x)[N], const AkvPack<T, N>& w) {
+  if constexpr (sizeof(T) == 4) {
+    memcpy(x, &w, sizeof(x));
+  } else if constexpr (N == 1) {
+    T t;
+    memcpy(&t, &w, sizeof(t));
+    x[0] = to_f32<T>(t);
+  } else {
+    uint32_t u[N / 2];
+    memcpy(u, &w, sizeof(u));
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        x[2 * i] = __uint_as_float(u[i] << 16);
+        x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
+  }
+}
+
+// Rounds x to T (x holds the rounded values afterwards).
+template <typename T, int N>
+AKV_DEV AkvPack<T, N> akv_pack(float (&x)[N]) {
+  AkvPack<T, N> w;
+  T t[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    t[i] = from_f32<T>(x[i]);
+    x[i] = to_f32<T>(t[i]);
+  }
+  memcpy(&w, t, sizeof(w));
+  return w;
+}
 
 // Waits until the launches before this one in the stream have ended and their
 // writes can be seen; a launch without the programmatic attribute passes.

@@ -6,13 +6,18 @@
 //   sum_d P_d kmax_d + N_d kmin_d,  P_d = sum_heads max(q_d, 0), N_d = sum_heads min(q_d, 0):
 // two products per dimension whatever the group.
 //
-// Scores are held in 64 bits: which of two blocks is taken hangs on the last
-// places of their scores, and products of 16-bit numbers and their sums are
-// exact there, so the choice does not depend on the order of a sum.
+// A score is a number in 64 bits: which of two blocks is taken hangs on the
+// last places of their scores, and products of 16-bit numbers and their sums are
+// exact there, so the choice does not depend on the order of a sum.  But 64-bit
+// arithmetic on every block took 8 times the time that reading them does (212 us
+// for 171 MB of bounds), so k_score works in 32 bits and brings, beside each
+// score, the sum of its terms' magnitudes: the score is off by at most
+// (group + 32) * 2^-23 of that (each of a lane's at most 16 products and 5 sums,
+// and of the group's sums in the coefficients, is off by 2^-24 of its own).  Only the
+// blocks that this leaves on both sides of the border (a few, unless
+// blocks are alike) are scored again in 64 bits, by k_select.
 //
-// What bounds it: 2 head_dim elements read per block and key head.  (The conversions to 64
-// bits come near: 16 a clock and SM, against the 11 or so elements that HBM
-// brings in that clock.)
+// What bounds it: 2 head_dim elements read per block and key head.
 #include <climits>
 
 #include "akv_paged.cuh"
@@ -20,8 +25,8 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSelectThreads = 512;
-constexpr int kTask = 64;          // blocks per warp and task
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
+constexpr int kWindow = 32;        // blocks whose ids a warp holds
 constexpr int kSharedKeys = 8192;  // keys that k_select holds in shared memory
 constexpr double kLargest = 1.7976931348623157e308;
 
@@ -33,10 +38,18 @@ struct SelectParams {
   const void* q;
   int64_t q_row, q_head;
   int32_t group, keep, first, last;
-  uint64_t* keys;  // [rows][heads][width]
+  int32_t task;    // blocks that a warp takes for one row and head, a multiple of kWindow
+  float2* near;    // [rows][heads][width]: score and its terms' magnitudes, in 32 bits
+  uint64_t* keys;  // [rows][heads][width]: of blocks that were scored in 64 bits
   int32_t* selected;
   AkvStatus* st;
 };
+
+AKV_DEV float warp_max(float x) {
+#pragma unroll
+  for (int off = 16; off; off >>= 1) x = fmaxf(x, __shfl_xor_sync(kFullWarp, x, off));
+  return x;
+}
 
 AKV_DEV int32_t blocks_of(const SelectParams& p, int32_t s) {
   return static_cast<int32_t>((static_cast<int64_t>(akv_held(p.tab, p.kv.bs_log2, s)) + (1 << p.kv.bs_log2) - 1) >>
@@ -52,23 +65,25 @@ AKV_DEV uint64_t key_of(double x) {
 }
 
 template <typename T, int kE, int kJ>
-__global__ void __launch_bounds__(kThreads) k_score(SelectParams p) {
+__global__ void __launch_bounds__(kThreads, 2) k_score(SelectParams p) {
   if (akv_failed(p.st)) return;
+  using Word = AkvPack<T, kE>;
+  constexpr int kBytes = kE * kJ * static_cast<int>(sizeof(T)), kB = kBytes <= 16 ? 4 : 2;
   const int lane = threadIdx.x & 31, dim = p.kv.dim;
-  const int64_t groups = (p.tab.width + kTask - 1) / kTask;
+  const int64_t groups = (p.tab.width + p.task - 1) / p.task;
   const int64_t tasks = p.tab.rows * groups * p.kv.heads;
   const int64_t layer_bytes = 2ll * p.kv.row_bytes;
   for (int64_t t = blockIdx.x * (kThreads / 32ll) + threadIdx.x / 32; t < tasks; t += gridDim.x * (kThreads / 32ll)) {
     const int32_t h = static_cast<int32_t>(t % p.kv.heads);
     const int32_t s = static_cast<int32_t>(t / p.kv.heads / groups);
-    const int32_t j0 = static_cast<int32_t>(t / p.kv.heads % groups) * kTask;
+    const int32_t j0 = static_cast<int32_t>(t / p.kv.heads % groups) * p.task;
     const int32_t n = blocks_of(p, s);
     if (n <= p.keep || j0 >= n) continue;
-    double coef[kJ * kE];
+    float coef[kJ * kE];
 #pragma unroll
     for (int j = 0; j < kJ; ++j)
 #pragma unroll
-      for (int i = 0; i < kE; ++i) coef[j * kE + i] = 0.0;
+      for (int i = 0; i < kE; ++i) coef[j * kE + i] = 0.f;
     for (int32_t g = 0; g < p.group; ++g) {
       const T* row = static_cast<const T*>(p.q) + s * p.q_row + (static_cast<int64_t>(h) * p.group + g) * p.q_head;
 #pragma unroll
@@ -79,130 +94,172 @@ __global__ void __launch_bounds__(kThreads) k_score(SelectParams p) {
 #pragma unroll
           for (int i = 0; i < kE; ++i) {
             const float q = to_f32<T>(row[(high ? at - dim : at) + i]);
-            coef[j * kE + i] += q != q ? static_cast<double>(q) : high ? fmax(q, 0.f) : fmin(q, 0.f);
+            coef[j * kE + i] += q != q ? q : high ? fmaxf(q, 0.f) : fminf(q, 0.f);
           }
         }
       }
     }
     const char* base = p.bounds + h * layer_bytes;
-    const int32_t stop = n - j0 < kTask ? n - j0 : kTask;
-    for (int32_t c0 = 0; c0 < stop; c0 += 32) {
-      int32_t id = 0;
-      if (c0 + lane < stop) {
-        id = p.tab.ids[s * p.tab.stride + j0 + c0 + lane];
-        if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.kv.total)) {
-          if (h == 0) akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, id, p.kv.total);
-          id = 0;
+    const int32_t stop = n - j0 < p.task ? n - j0 : p.task;
+    auto id_of = [&](int32_t c) -> int32_t {
+      if (c >= stop) return 0;
+      const int32_t id = p.tab.ids[s * p.tab.stride + j0 + c];
+      if (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.kv.total)) return id;
+      if (h == 0) akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, id, p.kv.total);
+      return 0;
+    };
+    int32_t id = id_of(lane), later = id_of(lane + kWindow);  // of this window and the next
+    // kB blocks at a time, the next kB's bounds on their way (behind the row's
+    // last block: block 0's, whose scores go nowhere)
+    Word w[kB][kJ];
+    auto ask = [&](int32_t c, Word(&to)[kB][kJ]) {
+#pragma unroll
+      for (int u = 0; u < kB; ++u) {
+        const char* box = base + __shfl_sync(kFullWarp, id, c % kWindow + u) * p.bounds_page;
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          const int at = (j * 32 + lane) * kE;
+          if (at < 2 * dim) to[u][j] = akv_load<T, kE>(box + at * sizeof(T));
         }
       }
-      for (int32_t c = c0; c < c0 + 32 && c < stop; c += 8) {
-        double sum[8];
+    };
+    ask(0, w);
+    for (int32_t c = 0; c < stop; c += kB) {
+      Word ahead[kB][kJ];
+      if ((c + kB) % kWindow == 0) {
+        id = later;
+        later = id_of(c + kB + kWindow + lane);
+      }
+      if (c + kB < stop) ask(c + kB, ahead);
+      float sum[kB], all[kB];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const char* box = base + __shfl_sync(kFullWarp, id, c - c0 + u) * p.bounds_page;
-          sum[u] = 0.0;
-          if (c + u < stop) {
+      for (int u = 0; u < kB; ++u) {
+        sum[u] = all[u] = 0.f;
 #pragma unroll
-            for (int j = 0; j < kJ; ++j) {
-              const int at = (j * 32 + lane) * kE;
-              if (at < 2 * dim) {
-                const AkvVec<T, kE> w = *reinterpret_cast<const AkvVec<T, kE>*>(box + at * sizeof(T));
+        for (int j = 0; j < kJ; ++j)
+          if ((j * 32 + lane) * kE < 2 * dim) {
+            float x[kE];
+            akv_unpack<T, kE>(x, w[u][j]);
 #pragma unroll
-                for (int i = 0; i < kE; ++i)
-                  sum[u] = fma(coef[j * kE + i], static_cast<double>(to_f32<T>(w.v[i])), sum[u]);
-              }
+            for (int i = 0; i < kE; ++i) {
+              sum[u] = fmaf(coef[j * kE + i], x[i], sum[u]);
+              all[u] = fmaf(fabsf(coef[j * kE + i]), fabsf(x[i]), all[u]);
             }
           }
-        }
-        // sum u ends, whole, in lanes 4 u .. 4 u + 3, added in the same order for every u
-        int off = 16;
-#pragma unroll
-        for (int w = 4; w >= 1; w >>= 1, off >>= 1) {
-          const bool up = lane & off;
-#pragma unroll
-          for (int i = 0; i < w; ++i) {
-            const double send = up ? sum[i] : sum[i + w], keep = up ? sum[i + w] : sum[i];
-            sum[i] = keep + __shfl_xor_sync(kFullWarp, send, off);
-          }
-        }
-        sum[0] += __shfl_xor_sync(kFullWarp, sum[0], 2);
-        sum[0] += __shfl_xor_sync(kFullWarp, sum[0], 1);
-        const int32_t mine = c + lane / 4;
-        if (lane % 4 == 0 && mine < stop)
-          p.keys[(static_cast<int64_t>(s) * p.kv.heads + h) * p.tab.width + j0 + mine] = key_of(sum[0]);
       }
+      // sum u ends, whole, in lanes u * 32 / kB ..
+      int off = 16;
+#pragma unroll
+      for (int x = kB / 2; x >= 1; x >>= 1, off >>= 1) {
+        const bool up = lane & off;
+#pragma unroll
+        for (int i = 0; i < x; ++i) {
+          const float a = up ? sum[i] : sum[i + x], b = up ? all[i] : all[i + x];
+          sum[i] = (up ? sum[i + x] : sum[i]) + __shfl_xor_sync(kFullWarp, a, off);
+          all[i] = (up ? all[i + x] : all[i]) + __shfl_xor_sync(kFullWarp, b, off);
+        }
+      }
+#pragma unroll
+      for (int x = 16 / kB; x >= 1; x >>= 1) {
+        sum[0] += __shfl_xor_sync(kFullWarp, sum[0], x);
+        all[0] += __shfl_xor_sync(kFullWarp, all[0], x);
+      }
+      const int32_t mine = c + lane / (32 / kB);
+      if (lane % (32 / kB) == 0 && mine < stop)
+        p.near[(static_cast<int64_t>(s) * p.kv.heads + h) * p.tab.width + j0 + mine] = make_float2(sum[0], all[0]);
+#pragma unroll
+      for (int u = 0; u < kB; ++u)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) w[u][j] = ahead[u][j];
     }
   }
 }
 
-// One CTA per (row, key head): a radix selection finds the lowest key that is
-// taken, digit by digit from the highest bit in which the keys differ, until
-// a digit's keys are all taken; then one pass in order writes the places.
-__global__ void __launch_bounds__(kSelectThreads) k_select(SelectParams p) {
-  extern __shared__ __align__(16) uint64_t held[];
-  __shared__ uint64_t ends[2][kSelectThreads / 32];
-  __shared__ int32_t bins[256];
-  __shared__ int32_t found[2];  // digit, keys above it
-  __shared__ uint32_t counts[2][kSelectThreads / 32];
-  akv_grid_wait();
-  if (akv_failed(p.st)) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int32_t s = blockIdx.x / p.kv.heads;
-  const int32_t n = blocks_of(p, s);
-  int32_t* out = p.selected + static_cast<int64_t>(blockIdx.x) * p.keep;
-  if (tid == 0 && blockIdx.x % p.kv.heads == 0 && p.tab.lengths[s] > akv_held(p.tab, p.kv.bs_log2, s))
-    akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, p.tab.lengths[s], p.tab.width);
-  if (n <= p.keep) {
-    for (int32_t i = tid; i < p.keep; i += kSelectThreads) out[i] = i < n ? i : -1;
-    return;
+// A finite score in 32 bits as a whole number of the same order, and back.
+AKV_DEV uint32_t order_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+AKV_DEV float value_of(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
+
+// The score of one block in 64 bits (a warp together; in the same order for every block).
+template <typename T>
+AKV_DEV double exact_score(const SelectParams& p, int32_t s, int32_t h, int32_t j, int lane) {
+  int32_t id = p.tab.ids[s * p.tab.stride + j];
+  if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.kv.total)) id = 0;
+  const T* box = reinterpret_cast<const T*>(p.bounds + id * p.bounds_page + h * 2ll * p.kv.row_bytes);
+  const T* q = static_cast<const T*>(p.q) + s * p.q_row + static_cast<int64_t>(h) * p.group * p.q_head;
+  double sum = 0.0;
+  for (int d = lane; d < p.kv.dim; d += 32) {
+    double up = 0.0, down = 0.0;
+    for (int32_t g = 0; g < p.group; ++g) {
+      const float x = to_f32<T>(q[g * p.q_head + d]);
+      up += x != x ? x : fmaxf(x, 0.f);
+      down += x != x ? x : fminf(x, 0.f);
+    }
+    sum = fma(up, static_cast<double>(to_f32<T>(box[p.kv.dim + d])), sum);
+    sum = fma(down, static_cast<double>(to_f32<T>(box[d])), sum);
   }
-  const uint64_t* keys = p.keys + static_cast<int64_t>(blockIdx.x) * p.tab.width;
-  const bool local = n <= kSharedKeys;
-  const int32_t from = p.first, to = n - p.last;  // [from, to) are ranked
-  uint64_t lo = ~0ull, hi = 0;
-  for (int32_t j = from + tid; j < to; j += kSelectThreads) {
-    const uint64_t k = keys[j];
-    if (local) held[j] = k;
+#pragma unroll
+  for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(kFullWarp, sum, off);
+  return sum;
+}
+
+template <typename K>
+struct RadixShared {
+  K ends[2][kSelectWarps];
+  int32_t bins[256];
+  int32_t found[2];  // digit, keys above it
+};
+
+// Narrows [prefix, prefix | ~mask] down to the `need`-th highest of the keys that
+// each(f) calls f(key) for, digit by digit from the highest bit in which they
+// differ, until a digit's keys are all taken.  `need` becomes how many of the
+// range are; at least one is.
+template <typename K, class Each>
+AKV_DEV void radix(RadixShared<K>& sh, Each each, int32_t& need, K& mask, K& prefix) {
+  constexpr int kBits = 8 * sizeof(K);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  K lo = ~static_cast<K>(0), hi = 0;
+  each([&](K k) {
     lo = k < lo ? k : lo;
     hi = k > hi ? k : hi;
-  }
-#pragma unroll
-  for (int off = 16; off; off >>= 1) {
-    const uint64_t a = __shfl_xor_sync(kFullWarp, lo, off), b = __shfl_xor_sync(kFullWarp, hi, off);
-    lo = a < lo ? a : lo;
-    hi = b > hi ? b : hi;
-  }
+  });
+  auto spread = [&](int width) {
+    for (int off = width; off; off >>= 1) {
+      const K a = __shfl_xor_sync(kFullWarp, lo, off), b = __shfl_xor_sync(kFullWarp, hi, off);
+      lo = a < lo ? a : lo;
+      hi = b > hi ? b : hi;
+    }
+  };
+  spread(16);
+  __syncthreads();
   if (lane == 0) {
-    ends[0][warp] = lo;
-    ends[1][warp] = hi;
+    sh.ends[0][warp] = lo;
+    sh.ends[1][warp] = hi;
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kSelectThreads / 32; ++w) {
-    lo = ends[0][w] < lo ? ends[0][w] : lo;
-    hi = ends[1][w] > hi ? ends[1][w] : hi;
-  }
-  auto key = [&](int32_t j) { return local ? held[j] : keys[j]; };
-  // keys with (key & mask) == prefix are still in question, `need` of them are taken
-  int32_t need = p.keep - p.first - p.last;
-  int bit = lo == hi ? 0 : 64 - __clzll(static_cast<long long>(lo ^ hi));  // bits below this differ
-  uint64_t mask = bit == 64 ? 0 : ~0ull << bit, prefix = hi & mask;
-  while (bit > 0 && need > 0) {
+  lo = sh.ends[0][lane % kSelectWarps];
+  hi = sh.ends[1][lane % kSelectWarps];
+  spread(16);
+  int bit = lo == hi ? 0 : sizeof(K) == 8 ? 64 - __clzll(static_cast<long long>(lo ^ hi)) : 32 - __clz(static_cast<int>(lo ^ hi));
+  mask = bit == kBits ? 0 : ~static_cast<K>(0) << bit;
+  prefix = hi & mask;
+  while (bit > 0) {
     const int width = bit < 8 ? bit : 8;
     bit -= width;
-    if (tid < 256) bins[tid] = 0;
+    if (tid < 256) sh.bins[tid] = 0;
     __syncthreads();
-    for (int32_t j = from + tid; j < to; j += kSelectThreads) {
-      const uint64_t k = key(j);
-      if ((k & mask) == prefix) atomicAdd(&bins[(k >> bit) & ((1 << width) - 1)], 1);
-    }
+    each([&](K k) {
+      if ((k & mask) == prefix) atomicAdd(&sh.bins[static_cast<int>(k >> bit) & ((1 << width) - 1)], 1);
+    });
     __syncthreads();
     if (warp == 0) {
       // lane i: digits 255 - 8 i .. 248 - 8 i, highest first
       int32_t sum = 0, at[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        at[i] = bins[255 - 8 * lane - i];
+        at[i] = sh.bins[255 - 8 * lane - i];
         sum += at[i];
       }
       int32_t incl = sum;
@@ -216,52 +273,174 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(SelectParams p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (above < need && above + at[i] >= need) {
-            found[0] = 255 - 8 * lane - i;
-            found[1] = above;
+            sh.found[0] = 255 - 8 * lane - i;
+            sh.found[1] = above;
           }
           above += at[i];
         }
       }
     }
     __syncthreads();
-    const int32_t digit = found[0], count = bins[digit];
-    need -= found[1];
-    mask |= static_cast<uint64_t>((1 << width) - 1) << bit;
-    prefix |= static_cast<uint64_t>(digit) << bit;
+    const int32_t digit = sh.found[0], count = sh.bins[digit];
+    need -= sh.found[1];
+    mask |= static_cast<K>((1 << width) - 1) << bit;
+    prefix |= static_cast<K>(digit) << bit;
     __syncthreads();
     if (count == need) break;  // all of them
   }
-  // taken: keys above the prefix's range, and the first `need` of those in it
-  int32_t above = 0, equal = 0;
-  int flip = 0;
-  for (int32_t j0 = 0; j0 < n; j0 += kSelectThreads, flip ^= 1) {
-    const int32_t j = j0 + tid;
-    bool gt = false, eq = false;
-    if (j < n) {
-      if (j < from || j >= to) {
-        gt = true;
-      } else {
-        const uint64_t k = key(j) & mask;
-        gt = k > prefix;
-        eq = k == prefix;
+}
+
+// One CTA per (row, key head): the border in 32 bits by a radix selection, the
+// blocks that lie too near to it again in 64 bits and among them a second one;
+// then the places, in order.
+template <typename T>
+__global__ void __launch_bounds__(kSelectThreads) k_select(SelectParams p) {
+  extern __shared__ __align__(16) float held[];
+  __shared__ union {
+    RadixShared<uint32_t> near;
+    RadixShared<uint64_t> exact;
+  } radix_sh;
+  __shared__ int32_t counts[2][kSelectWarps];
+  __shared__ float top[kSelectWarps];
+  akv_grid_wait();
+  if (akv_failed(p.st)) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int32_t s = blockIdx.x / p.kv.heads, h = blockIdx.x % p.kv.heads;
+  const int32_t n = blocks_of(p, s);
+  int32_t* out = p.selected + static_cast<int64_t>(blockIdx.x) * p.keep;
+  if (tid == 0 && h == 0 && p.tab.lengths[s] > akv_held(p.tab, p.kv.bs_log2, s))
+    akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, p.tab.lengths[s], p.tab.width);
+  if (n <= p.keep) {
+    for (int32_t i = tid; i < p.keep; i += kSelectThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const float2* near = p.near + static_cast<int64_t>(blockIdx.x) * p.tab.width;
+  uint64_t* keys = p.keys + static_cast<int64_t>(blockIdx.x) * p.tab.width;
+  const bool local = n <= kSharedKeys;
+  const int32_t from = p.first, to = n - p.last;  // [from, to) are ranked
+  int32_t need = p.keep - p.first - p.last;
+  float most = 0.f;
+#pragma unroll 8
+  for (int32_t j = from + tid; j < to; j += kSelectThreads) {
+    const float2 x = __ldcg(near + j);
+    if (local) held[j] = x.x;
+    // (infinities and NaN make this +inf: every block is scored again)
+    most = fmaxf(most, isfinite(x.x) && isfinite(x.y) ? x.y : INFINITY);
+  }
+  most = warp_max(most);
+  if (lane == 0) top[warp] = most;
+  __syncthreads();
+  most = warp_max(top[lane % kSelectWarps]);
+  const float off = (p.group + 32) * 1.1920929e-7f * most + 1e-35f;  // no score is further off than that
+  auto score = [&](int32_t j) { return local ? held[j] : near[j].x; };
+  // scores above `high` are taken, below `low` not
+  float low = -INFINITY, high = INFINITY;
+  if (isfinite(off) && need > 0) {
+    uint32_t mask, prefix;
+    int32_t left = need;
+    radix<uint32_t>(
+        radix_sh.near,
+        [&](auto f) {
+#pragma unroll 4
+          for (int32_t j = from + tid; j < to; j += kSelectThreads) f(order_of(score(j)));
+        },
+        left, mask, prefix);
+    low = value_of(prefix) - 2.f * off;
+    high = value_of(prefix | ~mask) + 2.f * off;
+    low -= fabsf(low) * 2.4e-7f;  // these two sums' own rounding
+    high += fabsf(high) * 2.4e-7f;
+    if (!(low > -INFINITY)) low = -INFINITY;
+    if (!(high < INFINITY)) high = INFINITY;
+  }
+  // Each warp counts its stretch.
+  const int32_t per = ((n + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
+  const int32_t w0 = warp * per, w1 = min(n, w0 + per);
+  // 2: taken, 1: in question, 0: not taken
+  auto class_of = [&](int32_t j) {
+    if (j < from || j >= to) return 2;
+    if (need == 0) return 0;
+    const float x = score(j);
+    return x > high ? 2 : x < low ? 0 : 1;
+  };
+  auto total = [&](int32_t* of) {  // of the warps' counts
+    int32_t x = of[lane % kSelectWarps];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFullWarp, x, o);
+    return x;
+  };
+  int32_t sure = 0, open = 0;
+  for (int32_t j = w0 + lane; j < w1; j += 32) {
+    const int c = class_of(j);
+    sure += c == 2;
+    open += c == 1;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    sure += __shfl_xor_sync(kFullWarp, sure, o);
+    open += __shfl_xor_sync(kFullWarp, open, o);
+  }
+  if (lane == 0) {
+    counts[0][warp] = sure;
+    counts[1][warp] = open;
+  }
+  __syncthreads();
+  int32_t left = p.keep - total(counts[0]);  // to take of those in question
+  const int32_t in_question = total(counts[1]);
+  uint64_t mask = 0, prefix = 0;  // (all of them equal)
+  if (left > 0 && left < in_question) {
+    for (int32_t j0 = w0; j0 < w1; j0 += 32) {
+      uint32_t open_here = __ballot_sync(kFullWarp, j0 + lane < w1 && class_of(j0 + lane) == 1);
+      for (; open_here; open_here &= open_here - 1) {
+        const int32_t j = j0 + __ffs(open_here) - 1;
+        const uint64_t k = key_of(exact_score<T>(p, s, h, j, lane));
+        if (lane == 0) keys[j] = k;
       }
     }
-    const uint32_t bg = __ballot_sync(kFullWarp, gt), be = __ballot_sync(kFullWarp, eq);
-    if (lane == 0) counts[flip][warp] = __popc(bg) | (__popc(be) << 16);
-    __syncthreads();
-    uint32_t before = 0, all = 0;
+    __syncthreads();  // (the keys are this CTA's own)
+    radix<uint64_t>(
+        radix_sh.exact,
+        [&](auto f) {
+          for (int32_t j = from + tid; j < to; j += kSelectThreads)
+            if (class_of(j) == 1) f(keys[j]);
+        },
+        left, mask, prefix);
+  }
+  // Taken: the sure ones, those in question above the prefix's range, and the
+  // first `left` of those in it.
+  auto classes = [&](int32_t j, uint32_t& gt, uint32_t& eq) {
+    const int c = j < w1 ? class_of(j) : 0;
+    const uint64_t k = c == 1 && mask != 0 ? keys[j] & mask : 0;
+    gt = __ballot_sync(kFullWarp, c == 2 || (c == 1 && k > prefix));
+    eq = __ballot_sync(kFullWarp, c == 1 && k == prefix);
+  };
+  int32_t above = 0, equal = 0;
+  for (int32_t j0 = w0; j0 < w1; j0 += 32) {
+    uint32_t gt, eq;
+    classes(j0 + lane, gt, eq);
+    above += __popc(gt);
+    equal += __popc(eq);
+  }
+  __syncthreads();
+  if (lane == 0) {
+    counts[0][warp] = above;
+    counts[1][warp] = equal;
+  }
+  __syncthreads();
+  above = lane < warp ? counts[0][lane % kSelectWarps] : 0;
+  equal = lane < warp ? counts[1][lane % kSelectWarps] : 0;
 #pragma unroll
-    for (int w = 0; w < kSelectThreads / 32; ++w) {
-      const uint32_t c = counts[flip][w];
-      before += w < warp ? c : 0;
-      all += c;
-    }
+  for (int o = 16; o; o >>= 1) {
+    above += __shfl_xor_sync(kFullWarp, above, o);
+    equal += __shfl_xor_sync(kFullWarp, equal, o);
+  }
+  for (int32_t j0 = w0; j0 < w1; j0 += 32) {
+    uint32_t gt, eq;
+    classes(j0 + lane, gt, eq);
     const uint32_t below = (1u << lane) - 1;
-    const int32_t g = above + static_cast<int32_t>(before & 0xffff) + __popc(bg & below);
-    const int32_t e = equal + static_cast<int32_t>(before >> 16) + __popc(be & below);
-    if (gt || (eq && e < need)) out[g + (e < need ? e : need)] = j;
-    above += static_cast<int32_t>(all & 0xffff);
-    equal += static_cast<int32_t>(all >> 16);
+    const int32_t g = above + __popc(gt & below), e = equal + __popc(eq & below);
+    if ((gt >> lane & 1) || ((eq >> lane & 1) && e < left)) out[g + min(e, left)] = j0 + lane;
+    above += __popc(gt);
+    equal += __popc(eq);
   }
 }
 
@@ -288,13 +467,11 @@ ScoreKernel score_kernel(int32_t dtype, int dim, int elements) {
 }
 
 int64_t key_bytes(int64_t rows, int64_t heads, int64_t width, int64_t keep) {
-  return width <= keep ? 0 : rows * heads * width * 8;
+  return width <= keep ? 0 : rows * heads * width * 16;
 }
 
-int allow_shared() {
-  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k_select),
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedKeys * 8);
-  return e == cudaSuccess ? AKV_OK : akv_cuda_fail(e, "k_select: shared memory");
+ScoreKernel select_kernel(int32_t dtype) {
+  return dtype == AKV_F32 ? k_select<float> : dtype == AKV_F16 ? k_select<__half> : k_select<__nv_bfloat16>;
 }
 
 }  // namespace
@@ -306,8 +483,10 @@ int akv_select_prepare() {
         if (int rc = akv_load_kernel(reinterpret_cast<const void*>(score_kernel(dtype, dim, elements)),
                                      "akv_prepare: k_score"))
           return rc;
-  if (int rc = akv_load_kernel(reinterpret_cast<const void*>(k_select), "akv_prepare: k_select")) return rc;
-  return allow_shared();
+  for (int32_t dtype : {AKV_F32, AKV_F16, AKV_BF16})
+    if (int rc = akv_load_kernel(reinterpret_cast<const void*>(select_kernel(dtype)), "akv_prepare: k_select"))
+      return rc;
+  return AKV_OK;
 }
 
 extern "C" int64_t akv_select_blocks_scratch_bytes(int32_t rows, int32_t num_kv_heads, int32_t table_width,
@@ -351,7 +530,8 @@ extern "C" int akv_select_blocks(const AkvPagedPool* pool, const void* bounds, c
   p.keep = keep;
   p.first = first;
   p.last = last;
-  p.keys = static_cast<uint64_t*>(scratch);
+  p.near = static_cast<float2*>(scratch);
+  p.keys = reinterpret_cast<uint64_t*>(p.near + need / 16);
   p.selected = selected;
   p.st = status;
   cudaStream_t st = akv_stream(stream);
@@ -366,17 +546,20 @@ extern "C" int akv_select_blocks(const AkvPagedPool* pool, const void* bounds, c
   if (need) {
     const uint64_t bits = reinterpret_cast<uintptr_t>(bounds) | static_cast<uint64_t>(p.kv.row_bytes);
     const int low = static_cast<int>(bits & (~bits + 1) & 31);
-    const int64_t warps = pairs * ((p.tab.width + kTask - 1) / kTask), per = kThreads / 32;
-    const int64_t ctas = (warps + per - 1) / per, most = 8ll * kAkvSMs;
+    // A task reads its row's queries and its first ids before it can start (3
+    // latencies): as many blocks each as leave every resident warp four, to even them out.
+    const int64_t per = kThreads / 32, most = 2ll * kAkvSMs;
+    const int64_t share = pairs * p.tab.width / (most * per * kWindow);
+    p.task = kWindow * static_cast<int32_t>(share < 8 ? 1 : share > 64 ? 16 : share / 4);
+    const int64_t warps = pairs * ((p.tab.width + p.task - 1) / p.task);
+    const int64_t ctas = (warps + per - 1) / per;
     score_kernel(pool->dtype, p.kv.dim, (low == 0 || low > 16 ? 16 : low) / es)<<<
         static_cast<unsigned>(ctas < most ? ctas : most), kThreads, 0, st>>>(p);
     AKV_LAUNCH_CHECK(what);
-    cfg.dynamicSmemBytes = static_cast<size_t>(p.tab.width < kSharedKeys ? p.tab.width : kSharedKeys) * 8;
+    cfg.dynamicSmemBytes = static_cast<size_t>(p.tab.width < kSharedKeys ? p.tab.width : kSharedKeys) * 4;
     cfg.numAttrs = 1;
-    if (cfg.dynamicSmemBytes > 48 * 1024)
-      if (int rc = allow_shared()) return rc;
   }
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, k_select, p);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, select_kernel(pool->dtype), p);
   if (err != cudaSuccess) return akv_cuda_fail(err, what);
   return AKV_OK;
 }
