@@ -4,7 +4,9 @@ Public API mirrors the reference package `agentkv`:
   AgentKVPool, DualRadixTree / CoWRadixTree, SlabAllocator, PoolConfig,
   AgentKVCache (the HuggingFace cache), BlockHandle, NodeHandle;
   kernels.copy_block / kernels.zero_block are the
-  drop-ins for agentkv.core.triton_kernels.  FanoutGraph replays a whole
+  drop-ins for agentkv.core.triton_kernels.  attention.kv_append /
+paged_attention / select_blocks decode on the pool's pages, DecodeBatch for
+many agents at once.  FanoutGraph replays a whole
   Tree-of-Thought fan-out (forks, copy-on-write copies, appends, frees) as
   one CUDA graph.
 
@@ -34,6 +36,7 @@ _EXPORTS = {
     "INVALID_NODE_ID": "radix_tree",
     "FanoutGraph": "fanout",
     "AgentKVCache": "hf_cache",
+    "DecodeBatch": "decode",
 }
 
 __all__ = ["__version__", *_EXPORTS]

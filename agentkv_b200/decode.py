@@ -1,0 +1,146 @@
+"""DecodeBatch — a set of agents decoding together on the pool's own pages.
+
+The reference's consumers hold one cache per agent and assemble its K and V
+for every layer (agentkv/hf_cache.py:57-153).  A DecodeBatch holds the block
+tables and lengths of many agents on the device, and a step of all of them is
+one ``advance`` (blocks allocated, shared ones copied on write, tables
+uploaded) and per layer one ``append`` and one ``attend``:
+
+    batch = pool.decode_batch([pool.fork(root) for _ in range(64)])
+    batch.advance([[t] for t in next_tokens])
+    for layer in range(num_layers):
+        q = batch.append(layer, k, v, query=q, rope=rope)   # k, v: [64, kv_heads, head_dim]
+        out = batch.attend(layer, q)                        # [64, heads, head_dim]
+
+The device tensors keep their addresses while the rows and the width do, so
+the calls of a step can be captured once and replayed after each ``advance``.
+"""
+
+from __future__ import annotations
+
+from typing import List, Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import attention as A
+from .radix_tree import NodeHandle
+
+
+class DecodeBatch:
+    """The agents `handles` of `pool`, whose tokens so far have their keys and
+    values in the pool, in that order; rows behind them, up to `rows`, are padding.
+    ``width`` is the blocks that a row's table has room for (grown as
+    needed when None).  With ``bounds`` (True, or a tensor that several
+    batches of the pool share; see attention.key_bounds) ``append`` keeps the
+    blocks' key bounds, which ``attend(keep=...)`` ranks them by; a new tensor
+    starts with the bounds of the blocks that the agents hold."""
+
+    def __init__(self, pool, handles: Sequence[NodeHandle], *, rows: Optional[int] = None, width: Optional[int] = None,
+                 bounds=None) -> None:
+        self.pool = pool
+        self.handles: List[NodeHandle] = list(handles)
+        n = len(self.handles)
+        self.rows = n if rows is None else int(rows)
+        if self.rows < n:
+            raise ValueError(f"DecodeBatch: {n} agents in {self.rows} rows")
+        if len({h.handle_id for h in self.handles}) != n:
+            raise ValueError("DecodeBatch: an agent appears twice")
+        self._fixed = width is not None
+        data = pool._allocator._kv_data
+        self._data = data
+        ids = [pool.get_block_ids(h) for h in self.handles]
+        need = max([len(b) for b in ids], default=0)
+        self.width = max(1, need) if width is None else int(width)
+        self.tables = torch.zeros((self.rows, self.width), dtype=torch.int32, device=data.device)
+        self.lengths = torch.zeros(self.rows, dtype=torch.int32, device=data.device)
+        self.starts: Optional[torch.Tensor] = None  # of the last advance, when a row got more or less than one token
+        self._upload(ids)
+        self.bounds: Optional[torch.Tensor] = None
+        if bounds is not None and bounds is not False:
+            if bounds is True:
+                n_blocks, layers, _, heads, _, dim = data.shape
+                self.bounds = torch.zeros((n_blocks, layers, heads, 2, dim), dtype=data.dtype, device=data.device)
+                for layer in range(layers):
+                    A.key_bounds(data, layer, self.tables, self.lengths, self.bounds)
+            else:
+                A._check_bounds(bounds, data, "DecodeBatch")
+                self.bounds = bounds
+
+    def _upload(self, ids: List[List[int]]) -> None:
+        need = max([len(b) for b in ids], default=0)
+        if need > self.width:
+            if self._fixed:
+                raise ValueError(f"DecodeBatch: a table of {self.width} blocks cannot hold {need}")
+            self.width = max(need, 2 * self.width)
+            self.tables = torch.zeros((self.rows, self.width), dtype=torch.int32, device=self.tables.device)
+        table = np.zeros((self.rows, self.width), np.int32)
+        for i, b in enumerate(ids):
+            table[i, : len(b)] = b
+        lens = np.zeros(self.rows, np.int32)
+        lens[: len(self.handles)] = [len(h.tokens) for h in self.handles]
+        # (from pageable memory: the copy has left these arrays when it returns)
+        self.tables.copy_(torch.from_numpy(table))
+        self.lengths.copy_(torch.from_numpy(lens))
+
+    def advance(self, tokens: Sequence[Sequence[int]]) -> None:
+        """Give agent i the new tokens ``tokens[i]`` (none: it sits this step
+        out): room is allocated, blocks that the new tokens go to are made
+        exclusive (copied when shared), and tables and lengths uploaded.  The
+        keys and values follow by ``append``, for every layer."""
+        if len(tokens) != len(self.handles):
+            raise ValueError(f"DecodeBatch.advance: tokens for {len(tokens)} of {len(self.handles)} agents")
+        pool, bs = self.pool, self.pool.block_size
+        counts = [len(t) for t in tokens]
+        if self._fixed:
+            for h, n in zip(self.handles, counts):
+                if len(h.tokens) + n > self.width * bs:
+                    raise ValueError(f"DecodeBatch: a table of {self.width} blocks cannot hold "
+                                     f"{len(h.tokens) + n} tokens")
+        writes = []
+        for h, n in zip(self.handles, counts):
+            if n == 0:
+                continue
+            first, shared = len(h.tokens) // bs, h.shared_match_len // bs
+            last = (len(h.tokens) + n - 1) // bs
+            if first < shared:
+                raise RuntimeError("Cannot overwrite shared prefix blocks!")
+            writes += [(h, b - shared) for b in range(first, last + 1)]
+        for h, n, new in zip(self.handles, counts, tokens):
+            if n:
+                required = (len(h.tokens) + n + bs - 1) // bs - len(pool.get_block_ids(h))
+                if required > 0:
+                    pool.allocate_blocks(h, required)
+        if writes:
+            pool.ensure_mutable_batch(writes)
+        for h, n, new in zip(self.handles, counts, tokens):
+            if n:
+                pool.append_tokens(h, list(new))
+        self._upload([pool.get_block_ids(h) for h in self.handles])
+        if all(n == 1 for n in counts):
+            self.starts = None
+        else:
+            starts = np.zeros(self.rows + 1, np.int32)
+            starts[1 : len(counts) + 1] = np.cumsum(counts)
+            starts[len(counts) + 1 :] = starts[len(counts)]
+            self.starts = torch.from_numpy(starts).to(self.lengths.device)
+
+    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, **kw) -> Optional[torch.Tensor]:
+        """attention.kv_append of the last advance's new tokens, all agents'
+        behind one another (one row per row of the batch where each got one): key and
+        value [tokens, kv_heads, head_dim]; ``query``, ``rope`` and the
+        rest as there.  Returns the rotated queries, if any."""
+        return A.kv_append(self._data, layer, key, value, self.tables, self.lengths, starts=self.starts,
+                           bounds=self.bounds, **kw)
+
+    def attend(self, layer: int, query: torch.Tensor, *, keep: int = 0, first: int = 1, last: int = 1, **kw):
+        """attention.paged_attention of one query per row, [rows, heads,
+        head_dim], over the row's tokens; with ``keep`` over the `keep` blocks
+        that attention.select_blocks picks (needs the batch's bounds)."""
+        if keep:
+            if self.bounds is None:
+                raise ValueError("DecodeBatch.attend: keep needs a batch with bounds")
+            kw["selected"] = A.select_blocks(query, self.bounds, layer, self.tables, self.lengths, keep,
+                                             block_size=self.pool.block_size, first=first, last=last,
+                                             status=kw.get("status"))
+        return A.paged_attention(query, self._data, layer, self.tables, self.lengths, **kw)

@@ -8,7 +8,8 @@ new tokens' rows and returns the layer's whole K and V.  The data movement is
 two launches per layer instead of a Python loop over tokens plus an indexing
 gather and a permute: akv_kv_scatter writes every new token's rows,
 akv_kv_gather assembles the contiguous [1, heads, tokens, head_dim] outputs
-straight from the block tiles.  The copy-on-write checks happen first, in the
+straight from the block tiles.  store() and attend() do without the second:
+the new tokens attend over the pool's blocks themselves.  The copy-on-write checks happen first, in the
 reference's order, as one batch: each block a new token starts (and the
 first new token's block) is checked before any row lands, which gives the
 reference's bytes because a copied block never holds rows of this update.
@@ -21,6 +22,7 @@ from typing import Any, Dict, Optional, Tuple
 import numpy as np
 import torch
 
+from . import attention as A
 from . import kernels as K
 from .pool import AgentKVPool
 from .radix_tree import NodeHandle
@@ -60,6 +62,8 @@ class AgentKVCache(DynamicCache):
         self._table_version = 0  # bumped whenever _table_dev is replaced
         self._slots_key: Optional[tuple] = None  # (first new token, count, table version) of _slots_dev
         self._slots_dev: Optional[torch.Tensor] = None
+        self._rows_key: Optional[tuple] = None  # (tokens held, queries) of _rows_len
+        self._rows_len: Optional[torch.Tensor] = None
 
     def get_seq_length(self, layer_idx: Optional[int] = 0) -> int:
         return self._seen_tokens
@@ -73,6 +77,47 @@ class AgentKVCache(DynamicCache):
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int,
                cache_kwargs: Optional[Dict[str, Any]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        table = self._write(key_states, value_states, layer_idx)
+        if self.append_only:
+            out_k, out_v = self._append(layer_idx, key_states, value_states, table)
+        else:
+            out_k, out_v = K.kv_gather(self.pool._allocator._kv_data, table, layer_idx, self._next_seen_tokens,
+                                       status=self.pool._allocator._status)
+        self._layer_done(layer_idx)
+        return out_k, out_v
+
+    def store(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
+        """update() without assembling the layer's K and V: for a model that
+        reads them where they lie, with attend() (called after store(), for
+        each layer)."""
+        self._write(key_states, value_states, layer_idx)
+        self._layer_done(layer_idx)
+
+    def attend(self, query: torch.Tensor, layer_idx: int, *, scale: Optional[float] = None,
+               window: int = 0) -> torch.Tensor:
+        """Causal attention of the last update's (or store's) n new tokens,
+        query [1, heads, n, head_dim] to the same shape, over the layer's blocks."""
+        if query.dim() != 4 or query.shape[0] != 1:
+            raise ValueError("AgentKVCache requires batch_size=1")
+        n = query.shape[2]
+        held = self._next_seen_tokens
+        if n > held or self._table_dev is None:
+            raise ValueError(f"AgentKVCache.attend: {n} queries over {held} tokens")
+        key = (held, n)
+        if self._rows_key != key:  # the same for every layer of a step
+            self._rows_len = torch.arange(held - n + 1, held + 1, dtype=torch.int32, device=query.device)
+            self._rows_key = key
+        out = A.paged_attention(query[0].transpose(0, 1), self.pool._allocator._kv_data, layer_idx,
+                                self._table_dev.expand(n, -1), self._rows_len, scale=scale, window=window)
+        return out.transpose(0, 1)[None]
+
+    def _layer_done(self, layer_idx: int) -> None:
+        if layer_idx == self.pool.config.num_layers - 1:
+            self._seen_tokens = self._next_seen_tokens
+
+    def _write(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> torch.Tensor:
+        """The new tokens' rows into the layer's blocks (allocated and made
+        exclusive on layer 0); returns the device block table."""
         if key_states.shape[0] != 1:
             raise ValueError("AgentKVCache requires batch_size=1")
         pool, h = self.pool, self.handle
@@ -107,13 +152,7 @@ class AgentKVCache(DynamicCache):
                 self._slots_dev = torch.from_numpy(slots.astype(np.int32)).to(kv.device)
                 self._slots_key = key
             K.kv_scatter(kv, self._slots_dev, layer_idx, key_states, value_states, status=st)
-        if self.append_only:
-            out_k, out_v = self._append(layer_idx, key_states, value_states, table)
-        else:
-            out_k, out_v = K.kv_gather(kv, table, layer_idx, self._next_seen_tokens, status=st)
-        if layer_idx == pool.config.num_layers - 1:
-            self._seen_tokens = self._next_seen_tokens
-        return out_k, out_v
+        return table
 
     def _append(self, layer: int, key_states: torch.Tensor, value_states: torch.Tensor,
                 table: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

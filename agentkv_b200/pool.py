@@ -3,7 +3,7 @@
 Thin delegation to DualRadixTree + SlabAllocator, exactly as in the reference,
 plus the batched entry points the device path makes cheap
 (``allocate_blocks``, ``fork_many``, ``ensure_mutable_batch``, ``free_many``,
-``match_prefix_batch``, ``match_prefix_many``).
+``match_prefix_batch``, ``match_prefix_many``, ``decode_batch``).
 """
 
 from __future__ import annotations
@@ -111,6 +111,13 @@ class AgentKVPool:
     def match_prefix_many(self, queries: Sequence) -> List[Tuple[Optional[NodeHandle], int]]:
         """The tree's match_prefix on every query (handles included), one lookup launch."""
         return self._tree.match_prefix_many(queries)
+
+    def decode_batch(self, handles: Sequence[NodeHandle], **kw):
+        """The agents as one DecodeBatch: their tables and lengths on the
+        device, appended to and attended over together."""
+        from .decode import DecodeBatch
+
+        return DecodeBatch(self, handles, **kw)
 
     def __repr__(self) -> str:
         s = self.stats()
