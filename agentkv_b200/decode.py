@@ -127,11 +127,14 @@ class DecodeBatch:
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, **kw) -> Optional[torch.Tensor]:
         """attention.kv_append of the last advance's new tokens, all agents'
-        behind one another (one row per row of the batch where each got one): key and
-        value [tokens, kv_heads, head_dim]; ``query``, ``rope`` and the
-        rest as there.  Returns the rotated queries, if any."""
-        return A.kv_append(self._data, layer, key, value, self.tables, self.lengths, starts=self.starts,
-                           bounds=self.bounds, **kw)
+        behind one another: key and value [tokens, kv_heads, head_dim] (where
+        each agent got one token: of the agents, or of all rows, padding
+        among them); ``query``, ``rope`` and the rest as there.  Returns the
+        rotated queries, if any."""
+        tables, lengths, n = self.tables, self.lengths, len(self.handles)
+        if self.starts is None and key.shape[0] == n < self.rows:
+            tables, lengths = tables[:n], lengths[:n]
+        return A.kv_append(self._data, layer, key, value, tables, lengths, starts=self.starts, bounds=self.bounds, **kw)
 
     def attend(self, layer: int, query: torch.Tensor, *, keep: int = 0, first: int = 1, last: int = 1, **kw):
         """attention.paged_attention of one query per row, [rows, heads,
