@@ -461,11 +461,13 @@ extern "C" int akv_kv_append(const AkvPagedPool* pool, const AkvPageBatch* batch
   // a row's n tokens lie in at most n, and at most n / block_size + 2, blocks
   const int64_t most = n_tokens / pool->block_size + 2ll * p.tab.rows;
   const int64_t units = starts == nullptr ? p.tab.rows : most < n_tokens ? most : n_tokens;
-  // as many CTAs per unit as its words fill, while there are SMs for them
+  // As many CTAs per unit as its words fill, while all are resident (2 an SM):
+  // a CTA has four latencies behind it (its row, its block, then words) before
+  // the first word moves, so waves of them cost more than a longer loop.
   const int64_t words = p.kv.dim / elements;
   const int64_t items = words * (8ll * p.kv.heads + (starts ? 4ll : 1ll) * p.q_heads / kHeads);
   int64_t per = (items + kThreads - 1) / kThreads;
-  const int64_t room = (8ll * kAkvSMs + units - 1) / units;
+  const int64_t room = 2ll * kAkvSMs / units;
   per = per < room ? per : room;
   const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(per < 1 ? 1 : per > 65535 ? 65535 : per));
   append_kernel(pool->dtype, elements)<<<grid, kThreads, 0, akv_stream(stream)>>>(p);

@@ -10,8 +10,8 @@
 // last places of their scores, and products of 16-bit numbers and their sums are
 // exact there, so the choice does not depend on the order of a sum.  But 64-bit
 // arithmetic on every block took 8 times the time that reading them does (212 us
-// for 171 MB of bounds), so k_score works in 32 bits and brings, beside each
-// score, the sum of its terms' magnitudes: the score is off by at most
+// for 171 MB of bounds), so k_score works in 32 bits and brings, beside the
+// scores, a bound on the sum of their terms' magnitudes: a score is off by at most
 // (group + 32) * 2^-23 of that (each of a lane's at most 16 products and 5 sums,
 // and of the group's sums in the coefficients, is off by 2^-24 of its own).  Only the
 // blocks that this leaves on both sides of the border (a few, unless
@@ -25,7 +25,6 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
 constexpr int kWindow = 32;        // blocks whose ids a warp holds
 constexpr int kSharedKeys = 8192;  // keys that k_select holds in shared memory
 constexpr double kLargest = 1.7976931348623157e308;
@@ -38,16 +37,30 @@ struct SelectParams {
   const void* q;
   int64_t q_row, q_head;
   int32_t group, keep, first, last;
+  int32_t q_words;  // the queries allow loads of whole words
   int32_t task;    // blocks that a warp takes for one row and head, a multiple of kWindow
-  float2* near;    // [rows][heads][width]: score and its terms' magnitudes, in 32 bits
+  float* near;     // [rows][heads][width]: scores in 32 bits
+  float* most;     // [rows][heads][tasks of a row]: what their terms' magnitudes add up to at most
   uint64_t* keys;  // [rows][heads][width]: of blocks that were scored in 64 bits
   int32_t* selected;
   AkvStatus* st;
 };
 
+AKV_DEV float max_nan(float a, float b) {  // NaN where either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+AKV_DEV float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 AKV_DEV float warp_max(float x) {
 #pragma unroll
-  for (int off = 16; off; off >>= 1) x = fmaxf(x, __shfl_xor_sync(kFullWarp, x, off));
+  for (int off = 16; off; off >>= 1) x = max_nan(x, __shfl_xor_sync(kFullWarp, x, off));
   return x;
 }
 
@@ -68,7 +81,7 @@ template <typename T, int kE, int kJ>
 __global__ void __launch_bounds__(kThreads, 2) k_score(SelectParams p) {
   if (akv_failed(p.st)) return;
   using Word = AkvPack<T, kE>;
-  constexpr int kBytes = kE * kJ * static_cast<int>(sizeof(T)), kB = kBytes <= 16 ? 4 : 2;
+  constexpr int kBytes = kE * kJ * static_cast<int>(sizeof(T)), kB = kBytes <= 16 ? 8 : kBytes <= 32 ? 4 : 2;
   const int lane = threadIdx.x & 31, dim = p.kv.dim;
   const int64_t groups = (p.tab.width + p.task - 1) / p.task;
   const int64_t tasks = p.tab.rows * groups * p.kv.heads;
@@ -79,7 +92,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_score(SelectParams p) {
     const int32_t j0 = static_cast<int32_t>(t / p.kv.heads % groups) * p.task;
     const int32_t n = blocks_of(p, s);
     if (n <= p.keep || j0 >= n) continue;
-    float coef[kJ * kE];
+    float coef[kJ * kE], most = 0.f;  // (the sum of the lanes' greatest is no less than any block's sum)
 #pragma unroll
     for (int j = 0; j < kJ; ++j)
 #pragma unroll
@@ -91,11 +104,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_score(SelectParams p) {
         const int at = (j * 32 + lane) * kE;
         if (at < 2 * dim) {
           const bool high = at >= dim;
+          const T* from = row + (high ? at - dim : at);
+          float q[kE];
+          if (p.q_words) {
+            akv_unpack<T, kE>(q, akv_load<T, kE>(from));
+          } else {
 #pragma unroll
-          for (int i = 0; i < kE; ++i) {
-            const float q = to_f32<T>(row[(high ? at - dim : at) + i]);
-            coef[j * kE + i] += q != q ? q : high ? fmaxf(q, 0.f) : fminf(q, 0.f);
+            for (int i = 0; i < kE; ++i) q[i] = to_f32<T>(from[i]);
           }
+#pragma unroll
+          for (int i = 0; i < kE; ++i) coef[j * kE + i] += high ? max_nan(q[i], 0.f) : min_nan(q[i], 0.f);
         }
       }
     }
@@ -131,10 +149,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_score(SelectParams p) {
         later = id_of(c + kB + kWindow + lane);
       }
       if (c + kB < stop) ask(c + kB, ahead);
-      float sum[kB], all[kB];
+      float sum[kB];
 #pragma unroll
       for (int u = 0; u < kB; ++u) {
-        sum[u] = all[u] = 0.f;
+        float all = 0.f;
+        sum[u] = 0.f;
 #pragma unroll
         for (int j = 0; j < kJ; ++j)
           if ((j * 32 + lane) * kE < 2 * dim) {
@@ -143,9 +162,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_score(SelectParams p) {
 #pragma unroll
             for (int i = 0; i < kE; ++i) {
               sum[u] = fmaf(coef[j * kE + i], x[i], sum[u]);
-              all[u] = fmaf(fabsf(coef[j * kE + i]), fabsf(x[i]), all[u]);
+              all = fmaf(fabsf(coef[j * kE + i]), fabsf(x[i]), all);
             }
           }
+        if (c + u < stop) most = max_nan(most, all);
       }
       // sum u ends, whole, in lanes u * 32 / kB ..
       int off = 16;
@@ -154,24 +174,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_score(SelectParams p) {
         const bool up = lane & off;
 #pragma unroll
         for (int i = 0; i < x; ++i) {
-          const float a = up ? sum[i] : sum[i + x], b = up ? all[i] : all[i + x];
+          const float a = up ? sum[i] : sum[i + x];
           sum[i] = (up ? sum[i + x] : sum[i]) + __shfl_xor_sync(kFullWarp, a, off);
-          all[i] = (up ? all[i + x] : all[i]) + __shfl_xor_sync(kFullWarp, b, off);
         }
       }
 #pragma unroll
-      for (int x = 16 / kB; x >= 1; x >>= 1) {
-        sum[0] += __shfl_xor_sync(kFullWarp, sum[0], x);
-        all[0] += __shfl_xor_sync(kFullWarp, all[0], x);
-      }
+      for (int x = 16 / kB; x >= 1; x >>= 1) sum[0] += __shfl_xor_sync(kFullWarp, sum[0], x);
       const int32_t mine = c + lane / (32 / kB);
       if (lane % (32 / kB) == 0 && mine < stop)
-        p.near[(static_cast<int64_t>(s) * p.kv.heads + h) * p.tab.width + j0 + mine] = make_float2(sum[0], all[0]);
+        p.near[(static_cast<int64_t>(s) * p.kv.heads + h) * p.tab.width + j0 + mine] = sum[0];
 #pragma unroll
       for (int u = 0; u < kB; ++u)
 #pragma unroll
         for (int j = 0; j < kJ; ++j) w[u][j] = ahead[u][j];
     }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) most += __shfl_xor_sync(kFullWarp, most, off);
+    if (lane == 0) p.most[(static_cast<int64_t>(s) * p.kv.heads + h) * groups + j0 / p.task] = most;
   }
 }
 
@@ -205,7 +224,7 @@ AKV_DEV double exact_score(const SelectParams& p, int32_t s, int32_t h, int32_t 
   return sum;
 }
 
-template <typename K>
+template <typename K, int kSelectWarps>
 struct RadixShared {
   K ends[2][kSelectWarps];
   int32_t bins[256];
@@ -214,10 +233,11 @@ struct RadixShared {
 
 // Narrows [prefix, prefix | ~mask] down to the `need`-th highest of the keys that
 // each(f) calls f(key) for, digit by digit from the highest bit in which they
-// differ, until a digit's keys are all taken.  `need` becomes how many of the
+// differ, until a digit's keys are all taken (kWhole: down to one key's
+// value, so that few lie too near to it).  `need` becomes how many of the
 // range are; at least one is.
-template <typename K, class Each>
-AKV_DEV void radix(RadixShared<K>& sh, Each each, int32_t& need, K& mask, K& prefix) {
+template <bool kWhole, typename K, int kSelectWarps, class Each>
+AKV_DEV void radix(RadixShared<K, kSelectWarps>& sh, Each each, int32_t& need, K& mask, K& prefix) {
   constexpr int kBits = 8 * sizeof(K);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   K lo = ~static_cast<K>(0), hi = 0;
@@ -286,19 +306,20 @@ AKV_DEV void radix(RadixShared<K>& sh, Each each, int32_t& need, K& mask, K& pre
     mask |= static_cast<K>((1 << width) - 1) << bit;
     prefix |= static_cast<K>(digit) << bit;
     __syncthreads();
-    if (count == need) break;  // all of them
+    if (!kWhole && count == need) break;  // all of them
   }
 }
 
 // One CTA per (row, key head): the border in 32 bits by a radix selection, the
 // blocks that lie too near to it again in 64 bits and among them a second one;
 // then the places, in order.
-template <typename T>
+template <typename T, int kSelectThreads>
 __global__ void __launch_bounds__(kSelectThreads) k_select(SelectParams p) {
+  constexpr int kSelectWarps = kSelectThreads / 32;
   extern __shared__ __align__(16) float held[];
   __shared__ union {
-    RadixShared<uint32_t> near;
-    RadixShared<uint64_t> exact;
+    RadixShared<uint32_t, kSelectWarps> near;
+    RadixShared<uint64_t, kSelectWarps> exact;
   } radix_sh;
   __shared__ int32_t counts[2][kSelectWarps];
   __shared__ float top[kSelectWarps];
@@ -314,31 +335,32 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(SelectParams p) {
     for (int32_t i = tid; i < p.keep; i += kSelectThreads) out[i] = i < n ? i : -1;
     return;
   }
-  const float2* near = p.near + static_cast<int64_t>(blockIdx.x) * p.tab.width;
+  const float* near = p.near + static_cast<int64_t>(blockIdx.x) * p.tab.width;
   uint64_t* keys = p.keys + static_cast<int64_t>(blockIdx.x) * p.tab.width;
   const bool local = n <= kSharedKeys;
   const int32_t from = p.first, to = n - p.last;  // [from, to) are ranked
   int32_t need = p.keep - p.first - p.last;
-  float most = 0.f;
+  if (local)
 #pragma unroll 8
-  for (int32_t j = from + tid; j < to; j += kSelectThreads) {
-    const float2 x = __ldcg(near + j);
-    if (local) held[j] = x.x;
-    // (infinities and NaN make this +inf: every block is scored again)
-    most = fmaxf(most, isfinite(x.x) && isfinite(x.y) ? x.y : INFINITY);
-  }
+    for (int32_t j = from + tid; j < to; j += kSelectThreads) held[j] = __ldcg(near + j);
+  // (with infinities and NaN among the terms this is none that is finite: every
+  // block is scored again)
+  float most = 0.f;
+  const int32_t tasks = (p.tab.width + p.task - 1) / p.task, used = (n + p.task - 1) / p.task;
+  for (int32_t i = tid; i < used; i += kSelectThreads)
+    most = max_nan(most, __ldcg(p.most + static_cast<int64_t>(blockIdx.x) * tasks + i));
   most = warp_max(most);
   if (lane == 0) top[warp] = most;
   __syncthreads();
   most = warp_max(top[lane % kSelectWarps]);
   const float off = (p.group + 32) * 1.1920929e-7f * most + 1e-35f;  // no score is further off than that
-  auto score = [&](int32_t j) { return local ? held[j] : near[j].x; };
+  auto score = [&](int32_t j) { return local ? held[j] : __ldcg(near + j); };
   // scores above `high` are taken, below `low` not
   float low = -INFINITY, high = INFINITY;
   if (isfinite(off) && need > 0) {
     uint32_t mask, prefix;
     int32_t left = need;
-    radix<uint32_t>(
+    radix<true>(
         radix_sh.near,
         [&](auto f) {
 #pragma unroll 4
@@ -363,7 +385,7 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(SelectParams p) {
     return x > high ? 2 : x < low ? 0 : 1;
   };
   auto total = [&](int32_t* of) {  // of the warps' counts
-    int32_t x = of[lane % kSelectWarps];
+    int32_t x = lane < kSelectWarps ? of[lane] : 0;
 #pragma unroll
     for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(kFullWarp, x, o);
     return x;
@@ -397,7 +419,7 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(SelectParams p) {
       }
     }
     __syncthreads();  // (the keys are this CTA's own)
-    radix<uint64_t>(
+    radix<false>(
         radix_sh.exact,
         [&](auto f) {
           for (int32_t j = from + tid; j < to; j += kSelectThreads)
@@ -467,11 +489,12 @@ ScoreKernel score_kernel(int32_t dtype, int dim, int elements) {
 }
 
 int64_t key_bytes(int64_t rows, int64_t heads, int64_t width, int64_t keep) {
-  return width <= keep ? 0 : rows * heads * width * 16;
+  return width <= keep ? 0 : rows * heads * width * 16;  // a key, a score and (at most one a block) a bound each
 }
 
+template <int kN>
 ScoreKernel select_kernel(int32_t dtype) {
-  return dtype == AKV_F32 ? k_select<float> : dtype == AKV_F16 ? k_select<__half> : k_select<__nv_bfloat16>;
+  return dtype == AKV_F32 ? k_select<float, kN> : dtype == AKV_F16 ? k_select<__half, kN> : k_select<__nv_bfloat16, kN>;
 }
 
 }  // namespace
@@ -484,8 +507,8 @@ int akv_select_prepare() {
                                      "akv_prepare: k_score"))
           return rc;
   for (int32_t dtype : {AKV_F32, AKV_F16, AKV_BF16})
-    if (int rc = akv_load_kernel(reinterpret_cast<const void*>(select_kernel(dtype)), "akv_prepare: k_select"))
-      return rc;
+    for (ScoreKernel k : {select_kernel<512>(dtype), select_kernel<1024>(dtype)})
+      if (int rc = akv_load_kernel(reinterpret_cast<const void*>(k), "akv_prepare: k_select")) return rc;
   return AKV_OK;
 }
 
@@ -530,14 +553,19 @@ extern "C" int akv_select_blocks(const AkvPagedPool* pool, const void* bounds, c
   p.keep = keep;
   p.first = first;
   p.last = last;
-  p.near = static_cast<float2*>(scratch);
-  p.keys = reinterpret_cast<uint64_t*>(p.near + need / 16);
+  p.keys = static_cast<uint64_t*>(scratch);
+  p.near = reinterpret_cast<float*>(p.keys + need / 16);
+  p.most = p.near + need / 16;
   p.selected = selected;
   p.st = status;
   cudaStream_t st = akv_stream(stream);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(pairs));
-  cfg.blockDim = dim3(kSelectThreads);
+  // 1,024 threads fill an SM: while there is one for each pair they finish
+  // sooner (19.5 against 24.8 us for 8 pairs of 8,126 blocks); beyond it two
+  // CTAs of 512 an SM do (21 against 25 us for 256 pairs of 560 to 2,048).
+  const bool few = pairs <= kAkvSMs;
+  cfg.blockDim = dim3(few ? 1024 : 512);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -546,6 +574,8 @@ extern "C" int akv_select_blocks(const AkvPagedPool* pool, const void* bounds, c
   if (need) {
     const uint64_t bits = reinterpret_cast<uintptr_t>(bounds) | static_cast<uint64_t>(p.kv.row_bytes);
     const int low = static_cast<int>(bits & (~bits + 1) & 31);
+    p.q_words = ((reinterpret_cast<uintptr_t>(query->data) | static_cast<uint64_t>(query->stride_token * es) |
+                  static_cast<uint64_t>(query->stride_head * es)) % 16) == 0;
     // A task reads its row's queries and its first ids before it can start (3
     // latencies): as many blocks each as leave every resident warp four, to even them out.
     const int64_t per = kThreads / 32, most = 2ll * kAkvSMs;
@@ -559,7 +589,7 @@ extern "C" int akv_select_blocks(const AkvPagedPool* pool, const void* bounds, c
     cfg.dynamicSmemBytes = static_cast<size_t>(p.tab.width < kSharedKeys ? p.tab.width : kSharedKeys) * 4;
     cfg.numAttrs = 1;
   }
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, select_kernel(pool->dtype), p);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, few ? select_kernel<1024>(pool->dtype) : select_kernel<512>(pool->dtype), p);
   if (err != cudaSuccess) return akv_cuda_fail(err, what);
   return AKV_OK;
 }
