@@ -48,7 +48,8 @@ _COUNTERS: dict = {}
 _POOL = struct.Struct("@Piiiiiiii").pack
 _BATCH = struct.Struct("@PPqii").pack
 _HEADS = struct.Struct("@Pqq").pack
-_capturing = torch.cuda.is_current_stream_capturing
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+_current_device = torch._C._cuda_getDevice
 
 
 def _status(device: torch.device, status: Optional[torch.Tensor], capturing: bool) -> Optional[torch.Tensor]:
@@ -79,17 +80,18 @@ def _counters(device: torch.device, stream: int, capturing: bool) -> torch.Tenso
     return buf
 
 
-def _pool_view(pool: torch.Tensor, layer: int, what: str) -> bytes:
-    """AkvPagedPool of one layer."""
+def _pool_view(pool: torch.Tensor, layer: int, what: str):
+    """AkvPagedPool of one layer, and the pool's heads, head_dim and type."""
     shape = pool.shape
     if len(shape) != 6 or shape[2] != 2 or not pool.is_contiguous():
         raise ValueError(f"{what}: pool must be a contiguous "
                          "[blocks, layers, 2, heads, block_size, head_dim] tensor")
-    dtype = _DTYPES.get(pool.dtype)
+    torch_dtype = pool.dtype
+    dtype = _DTYPES.get(torch_dtype)
     if dtype is None:
-        raise ValueError(f"{what}: pool dtype must be float16, bfloat16 or float32, got {pool.dtype}")
+        raise ValueError(f"{what}: pool dtype must be float16, bfloat16 or float32, got {torch_dtype}")
     n, layers, _, heads, bs, dim = shape
-    return _POOL(pool.data_ptr(), n, layers, heads, bs, dim, dtype, layer, 0)
+    return _POOL(pool.data_ptr(), n, layers, heads, bs, dim, dtype, layer, 0), heads, dim, torch_dtype
 
 
 def _batch_view(tables, lengths, device: torch.device, what: str):
@@ -112,17 +114,16 @@ def _batch_view(tables, lengths, device: torch.device, what: str):
     return _BATCH(tables.data_ptr(), lengths.data_ptr(), stride, width, rows), rows, width, tables, lengths
 
 
-def _heads_view(x: torch.Tensor, pool: torch.Tensor, name: str, what: str) -> bytes:
-    """AkvHeads of a [tokens, heads, head_dim] operand of the pool's (or the
-    bounds') head_dim, type and device."""
+def _heads_view(x: torch.Tensor, dim: int, dtype: torch.dtype, device: torch.device, name: str, what: str) -> bytes:
+    """AkvHeads of a [tokens, heads, head_dim] operand of the pool's head_dim, type and device."""
     shape = x.shape
-    if len(shape) != 3 or shape[2] != pool.shape[-1]:
-        raise ValueError(f"{what}: {name} must be [tokens, heads, {pool.shape[-1]}], got {tuple(x.shape)}")
-    if x.dtype != pool.dtype or x.device != pool.device:
-        raise ValueError(f"{what}: {name} must have the pool's dtype and device ({pool.dtype}, {pool.device}), "
+    if len(shape) != 3 or shape[2] != dim:
+        raise ValueError(f"{what}: {name} must be [tokens, heads, {dim}], got {tuple(shape)}")
+    if x.dtype != dtype or x.device != device:
+        raise ValueError(f"{what}: {name} must have the pool's dtype and device ({dtype}, {device}), "
                          f"got {x.dtype}, {x.device}")
     token, head, step = x.stride()
-    if step != 1 and shape[2] > 1:
+    if step != 1 and dim > 1:
         raise ValueError(f"{what}: {name}'s head_dim must be contiguous")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: {name} asks for a gradient; this is a forward-only operator")
@@ -130,7 +131,8 @@ def _heads_view(x: torch.Tensor, pool: torch.Tensor, name: str, what: str) -> by
 
 
 def _query_heads(query: torch.Tensor, pool_heads: int, what: str) -> int:
-    group, left = divmod(query.shape[1], pool_heads) if query.dim() == 3 else (0, 1)
+    shape = query.shape
+    group, left = divmod(shape[1], pool_heads) if len(shape) == 3 else (0, 1)
     if left or group == 0:
         raise ValueError(f"{what}: query must be [tokens, a multiple of {pool_heads} heads, head_dim], "
                          f"got {tuple(query.shape)}")
@@ -181,22 +183,13 @@ def _attention_scratch(geometry: bytes, rows: int, width: int, group: int, keep:
     return n
 
 
-class _On:
-    """The pool's device as the current one, when it is not (a launch goes to
-    the current device's context)."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, device: torch.device) -> None:
-        self.guard = None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
-
-    def __enter__(self) -> None:
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc) -> None:
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _on_device(device: torch.device, call):
+    """call() with the pool's device as the current one (a launch goes to the
+    current device's context)."""
+    if _current_device() == device.index:
+        return call()
+    with torch.cuda.device(device):
+        return call()
 
 
 def rope_table(rotary_dim: int, positions: int, *, theta: float = 10000.0, inv_freq: Optional[torch.Tensor] = None,
@@ -239,34 +232,37 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
     ([blocks, layers, heads, 2, head_dim], see key_bounds) is brought up to
     date for the blocks written."""
     what = "kv_append"
-    p = _pool_view(pool, layer, what)
-    H = pool.shape[3]
-    kview, vview = _heads_view(key, pool, "key", what), _heads_view(value, pool, "value", what)
-    tokens = key.shape[0]
-    if key.shape[1] != H or value.shape != key.shape:
-        raise ValueError(f"{what}: key and value must be [tokens, {H}, {pool.shape[5]}], got {tuple(key.shape)} "
+    p, H, dim, dtype = _pool_view(pool, layer, what)
+    dev = pool.device
+    kview, vview = _heads_view(key, dim, dtype, dev, "key", what), _heads_view(value, dim, dtype, dev, "value", what)
+    shape = key.shape
+    tokens = shape[0]
+    if shape[1] != H or value.shape != shape:
+        raise ValueError(f"{what}: key and value must be [tokens, {H}, {dim}], got {tuple(shape)} "
                          f"and {tuple(value.shape)}")
     qview = oview = None
     heads = 0
     if query is not None:
         _query_heads(query, H, what)
-        qview = _heads_view(query, pool, "query", what)
-        if query.shape[0] != tokens:
-            raise ValueError(f"{what}: {query.shape[0]} queries for {tokens} keys")
+        qview = _heads_view(query, dim, dtype, dev, "query", what)
+        qshape = query.shape
+        heads = qshape[1]
+        if qshape[0] != tokens:
+            raise ValueError(f"{what}: {qshape[0]} queries for {tokens} keys")
         if query_out is None:
-            query_out = query.new_empty(query.shape)
+            query_out = query.new_empty(qshape)
+            oview = _HEADS(query_out.data_ptr(), heads * dim, dim)
         elif query_out is not query:
             same = query_out.data_ptr() == query.data_ptr() and query_out.stride() == query.stride()
             _check_output(query_out, query, "query_out", what, key, value, pool, *(() if same else (query,)))
         if query_out is query:
             _check_output(query_out, query, "query_out", what, key, value, pool)
-        oview = _heads_view(query_out, pool, "query_out", what)
-        heads = query.shape[1]
+        if oview is None:
+            oview = _heads_view(query_out, dim, dtype, dev, "query_out", what)
     elif query_out is not None:
         raise ValueError(f"{what}: query_out without query")
-    if not _require_cuda(pool, what):
+    if not pool.is_cuda and not _require_cuda(pool, what):
         return query_out
-    dev = pool.device
     b, rows, _, tables, lengths = _batch_view(tables, lengths, dev, what)
     sptr = None
     if starts is not None:
@@ -287,7 +283,8 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
     if bounds is not None:
         _check_bounds(bounds, pool, what)
         bptr = bounds.data_ptr()
-    with _On(dev):
+
+    def call() -> None:
         st = _status(dev, status, _capturing())
         rc = N.lib.akv_kv_append(p, b, kview, vview, tokens, sptr, rptr, positions, rotary, interleaved, qview, oview,
                                  heads, bptr, None if st is None else st.data_ptr(), stream_handle(dev))
@@ -295,6 +292,8 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
             N.check(rc)
         if check and st is not None:
             raise_for_status(st)
+
+    _on_device(dev, call)
     return query_out
 
 
@@ -307,7 +306,7 @@ def key_bounds(pool: torch.Tensor, layer: int, tables, lengths, bounds: Optional
     tensor (zeros elsewhere) when none is given.  kv_append keeps bounds up to date by
     itself; this is for blocks that were written by other means."""
     what = "key_bounds"
-    p = _pool_view(pool, layer, what)
+    p = _pool_view(pool, layer, what)[0]
     n, L, _, H, _, D = pool.shape
     if bounds is None:
         bounds = torch.zeros((n, L, H, 2, D), dtype=pool.dtype, device=pool.device)
@@ -317,12 +316,15 @@ def key_bounds(pool: torch.Tensor, layer: int, tables, lengths, bounds: Optional
         return bounds
     dev = pool.device
     b, _, _, tables, lengths = _batch_view(tables, lengths, dev, what)
-    with _On(dev):
+
+    def call() -> None:
         st = _status(dev, status, _capturing())
         N.check(N.lib.akv_key_bounds(p, b, bounds.data_ptr(), None if st is None else st.data_ptr(),
                                      stream_handle(dev)))
         if check and st is not None:
             raise_for_status(st)
+
+    _on_device(dev, call)
     return bounds
 
 
@@ -348,18 +350,19 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, layer: int, tables,
     keep, first, last = int(keep), int(first), int(last)
     if keep < 1 or first < 0 or last < 0 or first + last > keep:
         raise ValueError(f"{what}: needs keep >= 1 and 0 <= first + last <= keep, got {keep}, {first}, {last}")
+    dev = bounds.device
     group = _query_heads(query, H, what)
-    qview = _heads_view(query, bounds, "query", what)
+    qview = _heads_view(query, D, bounds.dtype, dev, "query", what)
     rows = query.shape[0]
     selected = query.new_empty((rows, H, keep), dtype=torch.int32)
-    if not _require_cuda(bounds, what):
+    if not bounds.is_cuda and not _require_cuda(bounds, what):
         return selected
-    dev = bounds.device
     p = _POOL(0, n, L, H, block_size, D, dtype, layer, 0)
     b, batch, width, tables, lengths = _batch_view(tables, lengths, dev, what)
     if batch != rows:
         raise ValueError(f"{what}: {rows} queries for {batch} rows")
-    with _On(dev):
+
+    def call() -> None:
         st = _status(dev, status, _capturing())
         scratch = query.new_empty(max(0, N.lib.akv_select_blocks_scratch_bytes(rows, H, width, keep)),
                                   dtype=torch.uint8)
@@ -370,6 +373,8 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, layer: int, tables,
             N.check(rc)
         if check and st is not None:
             raise_for_status(st)
+
+    _on_device(dev, call)
     return selected
 
 
@@ -392,20 +397,20 @@ def paged_attention(query: torch.Tensor, pool: torch.Tensor, layer: int, tables,
     tokens of one sequence are several rows with the same table and
     their own lengths."""
     what = "paged_attention"
-    p = _pool_view(pool, layer, what)
-    group = _query_heads(query, pool.shape[3], what)
-    qview = _heads_view(query, pool, "query", what)
-    rows, heads, dim = query.shape
+    p, kv_heads, dim, dtype = _pool_view(pool, layer, what)
+    dev = pool.device
+    group = _query_heads(query, kv_heads, what)
+    qview = _heads_view(query, dim, dtype, dev, "query", what)
+    rows, heads, _ = query.shape
     if out is None:
         out = query.new_empty((rows, heads, dim))
         oview = _HEADS(out.data_ptr(), heads * dim, dim)
     else:
         _check_output(out, query, "out", what, query, pool)
-        oview = _heads_view(out, pool, "out", what)
+        oview = _heads_view(out, dim, dtype, dev, "out", what)
     lse = query.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
-    if not _require_cuda(pool, what):
+    if not pool.is_cuda and not _require_cuda(pool, what):
         return (out, lse) if return_lse else out
-    dev = pool.device
     window = int(window)
     if window < 0:
         raise ValueError(f"{what}: window must not be negative, got {window}")
@@ -415,12 +420,13 @@ def paged_attention(query: torch.Tensor, pool: torch.Tensor, layer: int, tables,
     sel, keep = None, 0
     if selected is not None:
         keep = selected.shape[-1] if selected.dim() == 3 else 0
-        if selected.shape != (rows, pool.shape[3], keep) or keep == 0 or selected.dtype != torch.int32 \
+        if selected.shape != (rows, kv_heads, keep) or keep == 0 or selected.dtype != torch.int32 \
                 or selected.device != dev or not selected.is_contiguous():
-            raise ValueError(f"{what}: selected must be a contiguous int32 [{rows}, {pool.shape[3]}, keep] tensor "
+            raise ValueError(f"{what}: selected must be a contiguous int32 [{rows}, {kv_heads}, keep] tensor "
                              f"on {dev}")
         sel = selected.data_ptr()
-    with _On(dev):
+
+    def call() -> None:
         capturing = _capturing()
         st, stream = _status(dev, status, capturing), stream_handle(dev)
         scratch = query.new_empty(_attention_scratch(p[8:], rows, width, group, keep), dtype=torch.uint8)
@@ -432,4 +438,6 @@ def paged_attention(query: torch.Tensor, pool: torch.Tensor, layer: int, tables,
             N.check(rc)
         if check and st is not None:
             raise_for_status(st)
+
+    _on_device(dev, call)
     return (out, lse) if return_lse else out
