@@ -44,7 +44,7 @@ ERROR_NAMES = {
 
 # ── element types (AKV_F32 ...) ───────────────────────────────────────────────
 F32, F16, BF16 = range(3)
-ATTENTION_COUNTERS = 1536  # AKV_ATTENTION_COUNTERS
+ATTENTION_COUNTERS = 1792  # AKV_ATTENTION_COUNTERS
 
 # ── ctl word indices ─────────────────────────────────────────────────────────
 CTL_FREE_LEFT = 0

@@ -18,7 +18,7 @@
 // the CTAs in equal contiguous ranges, whatever the rows' lengths are (the host
 // does not know them, and a captured launch replays with others).  A pair
 // inside one range is finished there; of one that crosses ranges each CTA
-// leaves a piece in scratch, and the last CTA to do so joins them (by 16s
+// leaves a piece in scratch, and the last CTA to do so joins them (by 20s
 // where there are more).
 #include <climits>
 
@@ -39,7 +39,7 @@ constexpr float kLowest = -3.402823466e38f;
 // 2^8 here), which spares most steps the reduction over the lanes.
 constexpr float kLazy = 8.0f;
 constexpr int kLeast = 2;                  // chunks per CTA: a piece costs as much as one or two
-constexpr int kFan = 16;                   // pieces that are joined at a time
+constexpr int kFan = 20;                   // pieces that are joined at a time
 constexpr int kMaxCtas = kFan * kFan * 2;  // two levels of joining
 
 struct AttendParams {
@@ -166,7 +166,7 @@ struct Cursor {
   }
 };
 
-// ── tensor-core engine: 16-bit types, head dims 64, 96, 128, 256 ────────────
+// ── tensor-core engine: 16-bit types, head dims that are whole 16-byte words ─
 // A warp takes 16 positions at a time with m16n8k16 products: S^T = K Q^T
 // (positions x heads), then O^T += V^T P^T (dimensions x heads); 8 query
 // heads are one product's width, so no row of a product is padding for a group
@@ -229,10 +229,12 @@ AKV_DEV float exp2_fast(float x) {
 AKV_DEV uint4 ld16(const char* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 AKV_DEV uint2 ld8(const char* p) { return __ldg(reinterpret_cast<const uint2*>(p)); }
 
-template <typename T, int kD, int kN>
+// Compiled for kD = 64, 96, 128 and 256; the dimensions between (kExact false) take the
+// next one's products with zeros behind their own words.
+template <typename T, int kD, int kN, bool kExact>
 struct MmaEngine {
   using Type = T;
-  static constexpr int kDim = kD;          // compiled for this head dim
+  static constexpr int kDim = kExact ? kD : 0;
   static constexpr int kCols = 8 * kN;     // query heads per pair
   static constexpr int kCtas = kD <= 128 && kN == 1 ? 3 : (kD <= 128 ? 2 : 1);
   static constexpr int kKi = kD / 32;      // 16-byte words of a key row per lane
@@ -247,21 +249,27 @@ struct MmaEngine {
   float o[kN][kMt][4];
   float m[kN][2], l[kN][2];
 
+  AKV_DEV static int row_of(const AttendParams& p) { return kExact ? kD * 2 : p.kv.row_bytes; }
+  // Whether word w (of `bytes` bytes) of a row is one of its own.
+  AKV_DEV static bool has(const AttendParams& p, int w, int bytes = 16) {
+    return kExact || w * bytes < p.kv.row_bytes;
+  }
+
   // Positions that take no part (bits of vm) are 0, whatever the block holds.
   AKV_DEV void load_k(const AttendParams& p, const Cursor& cur, const char* base, int32_t chunk, uint32_t vm,
                       int lane) {
     const int g = lane >> 2, c = lane & 3;
     const char *pa, *pb;
     if (p.kv.bs_log2 >= 3) {
-      pa = base + __shfl_sync(kFullWarp, cur.off, (chunk - cur.from) * 2) + g * (kD * 2);
-      pb = base + __shfl_sync(kFullWarp, cur.off, (chunk - cur.from) * 2 + 1) + g * (kD * 2);
+      pa = base + __shfl_sync(kFullWarp, cur.off, (chunk - cur.from) * 2) + g * row_of(p);
+      pb = base + __shfl_sync(kFullWarp, cur.off, (chunk - cur.from) * 2 + 1) + g * row_of(p);
     } else {
       pa = base + cur.row(p, chunk, g);
       pb = base + cur.row(p, chunk, g + 8);
     }
     pa += c * 16;
     pb += c * 16;
-    if (vm == 0xffffu) {
+    if (kExact && vm == 0xffffu) {
 #pragma unroll
       for (int i = 0; i < kKi; ++i) {
         ka[i] = ld16(pa + i * 64);
@@ -271,8 +279,8 @@ struct MmaEngine {
       const bool va = (vm >> g) & 1, vb = (vm >> (g + 8)) & 1;
 #pragma unroll
       for (int i = 0; i < kKi; ++i) {
-        ka[i] = va ? ld16(pa + i * 64) : make_uint4(0, 0, 0, 0);
-        kb[i] = vb ? ld16(pb + i * 64) : make_uint4(0, 0, 0, 0);
+        ka[i] = va && has(p, i * 4 + c) ? ld16(pa + i * 64) : make_uint4(0, 0, 0, 0);
+        kb[i] = vb && has(p, i * 4 + c) ? ld16(pb + i * 64) : make_uint4(0, 0, 0, 0);
       }
     }
   }
@@ -284,8 +292,8 @@ struct MmaEngine {
     if (p.kv.bs_log2 >= 3) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        row[2 * half] = base + __shfl_sync(kFullWarp, cur.off, (chunk - cur.from) * 2 + half) + c * (kD * 4);
-        row[2 * half + 1] = row[2 * half] + kD * 2;
+        row[2 * half] = base + __shfl_sync(kFullWarp, cur.off, (chunk - cur.from) * 2 + half) + c * 2 * row_of(p);
+        row[2 * half + 1] = row[2 * half] + row_of(p);
       }
     } else {
 #pragma unroll
@@ -296,8 +304,9 @@ struct MmaEngine {
       const int r = 2 * c + (x & 1) + (x >> 1) * 8;
       if (vm == 0xffffu || ((vm >> r) & 1)) {
 #pragma unroll
-        for (int i = 0; i < kVi; ++i) v[x][i] = ld16(row[x] + i * 128 + g * 16);
-        if (kVr) vr[x] = ld8(row[x] + kVi * 128 + g * 8);
+        for (int i = 0; i < kVi; ++i)
+          v[x][i] = has(p, i * 8 + g) ? ld16(row[x] + i * 128 + g * 16) : make_uint4(0, 0, 0, 0);
+        if (kVr) vr[x] = has(p, kVi * 16 + g, 8) ? ld8(row[x] + kVi * 128 + g * 8) : make_uint2(0, 0);
       } else {
 #pragma unroll
         for (int i = 0; i < kVi; ++i) v[x][i] = make_uint4(0, 0, 0, 0);
@@ -330,7 +339,8 @@ struct MmaEngine {
       const T* row = static_cast<const T*>(p.q) + s * p.q_row + (static_cast<int64_t>(h) * p.group + head) * p.q_head;
 #pragma unroll
       for (int i = 0; i < kKi; ++i)
-        q[n][i] = head < p.group ? ld16(reinterpret_cast<const char*>(row + i * 32 + c * 8)) : make_uint4(0, 0, 0, 0);
+        q[n][i] = head < p.group && has(p, i * 4 + c) ? ld16(reinterpret_cast<const char*>(row + i * 32 + c * 8))
+                                                      : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int t = 0; t < kMt; ++t)
 #pragma unroll
@@ -425,8 +435,8 @@ struct MmaEngine {
     }
   }
 
-  // This warp's sums: acc [kCols][kD], and m and l of each head.
-  AKV_DEV void store(float* acc, float2* ml, int /*dim*/, int lane) {
+  // This warp's sums: acc [kCols][dim], and m and l of each head.
+  AKV_DEV void store(float* acc, float2* ml, int dim, int lane) {
     const int g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int n = 0; n < kN; ++n)
@@ -440,7 +450,8 @@ struct MmaEngine {
 #pragma unroll
         for (int t = 0; t < kMt; ++t) {
           const int d = t < 4 * kVi ? (t >> 2) * 64 + g * 8 + 2 * (t & 3) : kVi * 64 + g * 4 + 2 * (t - 4 * kVi);
-          *reinterpret_cast<float2*>(acc + head * kD + d) = make_float2(o[n][t][x], o[n][t][x + 2]);
+          if (kExact || d < dim)
+            *reinterpret_cast<float2*>(acc + head * dim + d) = make_float2(o[n][t][x], o[n][t][x + 2]);
         }
       }
   }
@@ -458,7 +469,7 @@ struct SimtEngine {
   static constexpr int kDim = 0;
   static constexpr int kCols = kH;
   static constexpr int kX = kE * kJ;                      // dimensions per lane
-  static constexpr int kCtas = kH * kX * kL >= 32 * 32 ? 2 : 3;
+  static constexpr int kCtas = kH * kX * kL >= 32 * 32 ? 2 : kH * kX <= 8 ? 4 : 3;
   static constexpr int kSub = 32 / kL;                    // positions at a time
   static constexpr int kU = kL / kH < 4 || kX > 4 ? 2 : 4;
   static constexpr int kVals = kU * kH;                   // scores at a time,
@@ -823,7 +834,7 @@ __global__ void __launch_bounds__(kThreads, Eng::kCtas) k_attend(AttendParams p)
       finish_lses();
     } else {
       auto put = [&](int c, int d, float sum) { finish<T>(p, s, head0 + c, d, sum, joined[c].y); };
-      const int64_t first = c0 + (blockIdx.x - c0) / kFan * kFan;  // of this piece's sixteen
+      const int64_t first = c0 + (blockIdx.x - c0) / kFan * kFan;  // of this piece's twenty
       const int64_t near = min(static_cast<int64_t>(kFan), c1 + 1 - first), all = (c1 - c0) / kFan + 1;
       keep_ml(mine);
       if (last_of(p.arrived + 2 * first + (first == c0 ? 1 : 0), near)) {
@@ -861,39 +872,47 @@ Kernel kernel_of(const char* name) {
   return {k_attend<Eng>, Eng::kCols, Eng::kCtas, name};
 }
 
+template <typename T, int kD>
+Kernel mma_kernel(int dim, int group) {
+  // 16 heads of 256 dimensions do not fit the registers: two pairs of 8
+  if constexpr (kD < 256)
+    if (group > 8)
+      return dim == kD ? kernel_of<MmaEngine<T, kD, 2, true>>("mma x16") : kernel_of<MmaEngine<T, kD, 2, false>>("mma x16");
+  return dim == kD ? kernel_of<MmaEngine<T, kD, 1, true>>("mma x8") : kernel_of<MmaEngine<T, kD, 1, false>>("mma x8");
+}
+
 template <typename T>
 Kernel mma_kernel(int dim, int group) {
-  const bool wide = group > 8;
-  switch (dim) {
-    case 64: return wide ? kernel_of<MmaEngine<T, 64, 2>>("mma 64x16") : kernel_of<MmaEngine<T, 64, 1>>("mma 64x8");
-    case 96: return wide ? kernel_of<MmaEngine<T, 96, 2>>("mma 96x16") : kernel_of<MmaEngine<T, 96, 1>>("mma 96x8");
-    case 128: return wide ? kernel_of<MmaEngine<T, 128, 2>>("mma 128x16") : kernel_of<MmaEngine<T, 128, 1>>("mma 128x8");
-    // 16 heads of 256 dimensions do not fit the registers: two pairs of 8
-    case 256: return kernel_of<MmaEngine<T, 256, 1>>("mma 256x8");
-    default: return {};
-  }
+  return dim <= 64    ? mma_kernel<T, 64>(dim, group)
+         : dim <= 96  ? mma_kernel<T, 96>(dim, group)
+         : dim <= 128 ? mma_kernel<T, 128>(dim, group)
+                      : mma_kernel<T, 256>(dim, group);
 }
 
 // The widest word that the head dim and the addresses allow, at most 16
 // bytes and at most 4 elements, and no more lanes than a row fills.
+template <typename T, int kH>
+Kernel simt_kernel(int dim, int elements) {
+  if (elements >= 4 && dim % 4 == 0) {
+    if (dim <= 64) return kernel_of<SimtEngine<T, 4, 1, 16, kH>>("simt 64");
+    if (dim <= 128) return kernel_of<SimtEngine<T, 4, 1, 32, kH>>("simt 128");
+    return kernel_of<SimtEngine<T, 4, 2, 32, kH>>("simt 256");
+  }
+  return kernel_of<SimtEngine<T, 1, 8, 32, kH>>("simt");
+}
+
 template <typename T>
 Kernel simt_kernel(int dim, int group, int elements) {
-  const bool wide = group > 2;
-  if (elements >= 4 && dim % 4 == 0) {
-    if (dim <= 64) return wide ? kernel_of<SimtEngine<T, 4, 1, 16, 8>>("simt 64x8") : kernel_of<SimtEngine<T, 4, 1, 16, 2>>("simt 64x2");
-    if (dim <= 128) return wide ? kernel_of<SimtEngine<T, 4, 1, 32, 8>>("simt 128x8") : kernel_of<SimtEngine<T, 4, 1, 32, 2>>("simt 128x2");
-    return wide ? kernel_of<SimtEngine<T, 4, 2, 32, 8>>("simt 256x8") : kernel_of<SimtEngine<T, 4, 2, 32, 2>>("simt 256x2");
-  }
-  return wide ? kernel_of<SimtEngine<T, 1, 8, 32, 8>>("simt 1x8") : kernel_of<SimtEngine<T, 1, 8, 32, 2>>("simt 1x2");
+  return group <= 2   ? simt_kernel<T, 2>(dim, elements)
+         : group <= 4 ? simt_kernel<T, 4>(dim, elements)
+                      : simt_kernel<T, 8>(dim, elements);
 }
 
 // `align`: the power of two that divides every address and stride, in bytes.
 Kernel choose(int32_t dtype, int dim, int group, int align) {
   const int elements = align / akv_dtype_bytes(dtype);
   if (dtype == AKV_F32) return simt_kernel<float>(dim, group, elements);
-  Kernel k;
-  if (align >= 16) k = dtype == AKV_F16 ? mma_kernel<__half>(dim, group) : mma_kernel<__nv_bfloat16>(dim, group);
-  if (k.attend) return k;
+  if (align >= 16) return dtype == AKV_F16 ? mma_kernel<__half>(dim, group) : mma_kernel<__nv_bfloat16>(dim, group);
   return dtype == AKV_F16 ? simt_kernel<__half>(dim, group, elements) : simt_kernel<__nv_bfloat16>(dim, group, elements);
 }
 
@@ -904,7 +923,7 @@ int parts_of(const Kernel& k, int group) { return akv_ceil_div(group, k.cols); }
 // Grid of a launch over `rows` rows of at most `chunks` chunks each.
 int64_t grid_of(const Kernel& k, int64_t rows, int64_t pairs, int64_t chunks) {
   const int64_t most = rows * pairs * chunks, fit = static_cast<int64_t>(kAkvSMs) * k.ctas;
-  static_assert(kAkvSMs * 3 <= kMaxCtas && 3 * kMaxCtas <= AKV_ATTENTION_COUNTERS, "two levels of joining");
+  static_assert(kAkvSMs * 4 <= kMaxCtas && 3 * kAkvSMs * 4 <= AKV_ATTENTION_COUNTERS, "two levels of joining");
   return most < 1 ? 1 : (most < fit ? most : fit);
 }
 
@@ -965,8 +984,8 @@ int akv_tables_view(const char* what, const AkvPageBatch* b, int32_t block_size,
 
 int akv_attend_prepare() {
   for (int32_t dtype : {AKV_F32, AKV_F16, AKV_BF16})
-    for (int group : {1, 4, 9})
-      for (int dim : {60, 64, 96, 100, 128, 200, 256})
+    for (int group : {1, 4, 8, 9})
+      for (int dim : {56, 64, 80, 96, 104, 128, 200, 256})
         for (int align : {4, 16}) {
           const Kernel k = choose(dtype, dim, group, align);
           if (int rc = akv_load_kernel(reinterpret_cast<const void*>(k.attend), k.name)) return rc;

@@ -743,7 +743,7 @@ AKV_API int akv_key_bounds(const AkvPagedPool* pool, const AkvPageBatch* batch, 
  * not overlap on the GPU (one array per stream, one per captured call).  An id
  * out of range is reported (AKV_ERR_OUT_OF_RANGE) and its positions left out;
  * status is written only (an earlier error does not stop the call). */
-enum { AKV_ATTENTION_COUNTERS = 1536 };
+enum { AKV_ATTENTION_COUNTERS = 1792 };
 AKV_API int64_t akv_paged_attention_scratch_bytes(const AkvPagedPool* pool, int32_t rows, int32_t table_width,
                                           int32_t group, int32_t keep);
 AKV_API int akv_paged_attention(const AkvPagedPool* pool, const AkvPageBatch* batch, const AkvHeads* query,

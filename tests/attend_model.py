@@ -3,7 +3,7 @@ Python: how a batch's chunks are dealt to the CTAs, and which CTA joins which
 pieces.  Same names and the same rules, statement by statement where the result
 depends on them."""
 
-CHUNK, FAN, LEAST = 64, 16, 2
+CHUNK, FAN, LEAST = 64, 20, 2
 
 
 def extent(length, width, bs, window, keep):

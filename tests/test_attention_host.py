@@ -33,9 +33,9 @@ def test_every_chunk_is_read_once_and_every_piece_joined(seed):
 
 def test_two_levels_of_joining():
     """One pair over every CTA of the largest grid."""
-    reads, joins = M.simulate([444 * 2 * 64], 444 * 8, 16, 1, 1, 444)
-    assert len(reads) == 888 and sorted(joins[(0, 0)]) == list(range(444))
-    assert 3 * 444 <= N.ATTENTION_COUNTERS
+    reads, joins = M.simulate([592 * 2 * 64], 592 * 8, 16, 1, 1, 592)
+    assert len(reads) == 1184 and sorted(joins[(0, 0)]) == list(range(592))
+    assert 3 * 592 <= N.ATTENTION_COUNTERS
 
 
 @pytest.mark.parametrize("count", [1, 8])
