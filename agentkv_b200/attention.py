@@ -24,10 +24,11 @@ wait; its work space comes from PyTorch's allocator for that stream, so calls
 on several streams and captured calls do not share any.  Ids and lengths that
 only the device can check are reported in ``status`` (an AkvStatus record, by
 default one per device and stream, and one per device for captured calls;
-``check=True`` waits and raises): the tokens concerned are skipped, and
-calls behind them do nothing until the record is cleared (BlockOpError by
-``check=True`` clears it).  Forward only: an input that asks for a gradient is
-refused.
+``check=True`` waits and raises BlockOpError, which clears it).  The tokens
+concerned are left out; while the record holds an error, kv_append and
+key_bounds write nothing, as the framework's other writes (the reads go on).
+Make a call once before capturing it (a pool's allocator does that for all).
+Forward only: an input that asks for a gradient is refused.
 """
 
 from __future__ import annotations

@@ -79,7 +79,6 @@ AKV_DEV uint64_t key_of(double x) {
 
 template <typename T, int kE, int kJ>
 __global__ void __launch_bounds__(kThreads, 2) k_score(SelectParams p) {
-  if (akv_failed(p.st)) return;
   using Word = AkvPack<T, kE>;
   constexpr int kBytes = kE * kJ * static_cast<int>(sizeof(T)), kB = kBytes <= 16 ? 8 : kBytes <= 32 ? 4 : 2;
   const int lane = threadIdx.x & 31, dim = p.kv.dim;
@@ -324,7 +323,6 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(SelectParams p) {
   __shared__ int32_t counts[2][kSelectWarps];
   __shared__ float top[kSelectWarps];
   akv_grid_wait();
-  if (akv_failed(p.st)) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int32_t s = blockIdx.x / p.kv.heads, h = blockIdx.x % p.kv.heads;
   const int32_t n = blocks_of(p, s);

@@ -761,7 +761,8 @@ AKV_API int akv_paged_attention(const AkvPagedPool* pool, const AkvPageBatch* ba
  * `first` and the last `last` blocks (first + last <= keep) and the
  * highest-scored of the others, the lowest place of equal ones.  A NaN score
  * counts as the highest.  scratch: akv_select_blocks_scratch_bytes() bytes,
- * 16-byte aligned, as above. */
+ * 16-byte aligned, as above; status is written only, and a block whose id is out of
+ * range is ranked as block 0 is. */
 AKV_API int64_t akv_select_blocks_scratch_bytes(int32_t rows, int32_t num_kv_heads, int32_t table_width, int32_t keep);
 AKV_API int akv_select_blocks(const AkvPagedPool* pool, const void* bounds, const AkvPageBatch* batch,
                       const AkvHeads* query, int32_t group, int32_t keep, int32_t first, int32_t last,

@@ -259,6 +259,39 @@ def test_bad_ids_and_lengths_are_reported_and_left_out():
     assert torch.equal(_attend(q, pool, table, lens, 0), good)  # and the next call is whole again
 
 
+def test_nothing_to_do():
+    """No rows, tables of no width, batches of padding alone."""
+    pool = torch.zeros((4, 1, 2, 2, 16, 64), dtype=BF16, device=DEV)
+    bounds = torch.zeros((4, 1, 2, 2, 64), dtype=BF16, device=DEV)
+    for rows, width in ((0, 3), (3, 0), (3, 2)):
+        q = torch.ones(rows, 4, 64, dtype=BF16, device=DEV)
+        t = torch.zeros(rows, width, dtype=torch.int32, device=DEV)
+        n = torch.zeros(rows, dtype=torch.int32, device=DEV)
+        out, lse = A.paged_attention(q, pool, 0, t, n, return_lse=True, check=True)
+        assert out.shape == q.shape and (out == 0).all() and (lse == -math.inf).all()
+        sel = A.select_blocks(q, bounds, 0, t, n, 3, block_size=16, check=True)
+        assert sel.shape == (rows, 2, 3) and (sel == -1).all()
+        k = q[:, :2]
+        assert torch.equal(A.kv_append(pool, 0, k, k, t, n, query=q, query_out=q, check=True), q)
+        A.key_bounds(pool, 0, t, n, bounds, check=True)
+        assert (pool == 0).all() and (bounds == 0).all()
+
+
+def test_reads_go_on_behind_an_error():
+    pool, table, lens, g = _setup(BF16, 2, 64, 16, [40, 700], layers=1)
+    bounds = A.key_bounds(pool, 0, table, lens)
+    q = _randn(g, 2, 8, 64, dtype=BF16)
+    sel = A.select_blocks(q, bounds, 0, table, lens, 5, block_size=16)
+    out = _attend(q, pool, table, lens, 0, selected=sel)
+    st = torch.zeros(8, dtype=torch.int32, device=DEV)
+    st[0] = N.AKV_ERR_OUT_OF_RANGE
+    assert torch.equal(A.select_blocks(q, bounds, 0, table, lens, 5, block_size=16, status=st), sel)
+    assert torch.equal(A.paged_attention(q, pool, 0, table, lens, selected=sel, status=st), out)
+    before = pool.clone()
+    A.kv_append(pool, 0, q[:, :2], q[:, :2], table, lens, status=st)
+    assert torch.equal(pool.nan_to_num(3.0), before.nan_to_num(3.0))
+
+
 # ── append ───────────────────────────────────────────────────────────────────
 def _rotate64(x, pos, rot, interleaved, theta=10000.0):
     x = x.double().clone()
