@@ -94,8 +94,6 @@ AKV_DEV AkvPack<T, N> akv_pack(float (&x)[N]) {
 // Waits until the launches before this one in the stream have ended and their
 // writes can be seen; a launch without the programmatic attribute passes.
 AKV_DEV void akv_grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Lets the next launch of the stream begin (it waits as above before it reads).
-AKV_DEV void akv_grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // One layer of the pool [total][L][2][H][bs][D], in bytes.
 struct AkvLayer {

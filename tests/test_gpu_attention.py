@@ -272,6 +272,10 @@ def test_nothing_to_do():
         sel = A.select_blocks(q, bounds, 0, t, n, 3, block_size=16, check=True)
         assert sel.shape == (rows, 2, 3) and (sel == -1).all()
         k = q[:, :2]
+        if rows:  # the queries' result over the keys
+            with pytest.raises(ValueError, match="query_out shares memory"):
+                A.kv_append(pool, 0, k, k, t, n, query=q, query_out=q, check=True)
+            k = k.clone()
         assert torch.equal(A.kv_append(pool, 0, k, k, t, n, query=q, query_out=q, check=True), q)
         A.key_bounds(pool, 0, t, n, bounds, check=True)
         assert (pool == 0).all() and (bounds == 0).all()
