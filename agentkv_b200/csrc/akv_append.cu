@@ -13,7 +13,10 @@
 // Work: one unit per (row, block) that gets tokens, dealt to one or several
 // CTAs by words of kV elements (with the word of their partners); the four
 // lanes that hold a key's word bring its bounds together: no atomics, and the
-// same result in any order.
+// same result in any order.  Measured: 8,466 prompt tokens with 32 query and 8 key
+// heads of 128 in bf16 66 us (215 MB, 3.3 TB/s; the search, the table and the
+// loads come one after the other in a CTA, and 1.8 rounds of CTAs hide little of
+// it); 256 rows of one token 19 us, one row 10 us.
 #include <climits>
 
 #include "akv_paged.cuh"
@@ -21,7 +24,9 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;  // query heads that a thread turns together
+// Query heads that a thread turns together with one load of the angles.  2 with three
+// CTAs an SM spilled registers and took 98 us for the prompts, 4 with two take 66.
+constexpr int kHeads = 4;
 
 AKV_DEV int32_t akv_ceil_div_dev(int32_t a, int32_t b) { return (a + b - 1) / b; }
 

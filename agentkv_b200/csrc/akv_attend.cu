@@ -182,7 +182,8 @@ struct Cursor {
 // (Measured on 256 rows of 4,096 positions, 4.3 GB, where a plain read of the
 // same blocks takes 615 us: 16-byte asynchronous copies into shared memory
 // 846 us, bulk copies of whole blocks 765 us: their issue and the reads
-// from shared memory held the warps up more than the memory did.)
+// from shared memory held the warps up more than the memory did; this form
+// 639-667 us, 6.4-6.7 TB/s.  One row of 200,001 positions 138-144 us, 5.7-5.9 TB/s.)
 template <typename T>
 struct Pack2;
 template <>
@@ -462,7 +463,10 @@ struct MmaEngine {
 // between them, kE consecutive dimensions of every kL kE each, so a warp has
 // 32 / kL positions at a time; kU such steps give kU * kH partial scores per
 // lane, which halving exchanges turn into one whole score (or a copy) per
-// lane.  The next positions are loaded while these are computed.
+// lane.  The next positions are loaded while these are computed.  What bounds it:
+// latency, with 16 warps an SM (48 rows, window of 1,024, head dim 64: 35 us, 88 MB,
+// 2.5 TB/s; 41 us with three CTAs an SM instead of four; 16 rows of 8,000 at 128
+// dimensions 317 to 420 us, 3.3 to 2.5 TB/s).
 template <typename T, int kE, int kJ, int kL, int kH>
 struct SimtEngine {
   using Type = T;
@@ -874,7 +878,11 @@ Kernel kernel_of(const char* name) {
 
 template <typename T, int kD>
 Kernel mma_kernel(int dim, int group) {
-  // 16 heads of 256 dimensions do not fit the registers: two pairs of 8
+  // More than 8 heads: 16 columns read the keys once (8,000 positions of 16 rows,
+  // 16 heads of 128 in bf16, 114 us), two pairs of 8 twice (180).  16 heads of 256
+  // dimensions do not fit the registers: two pairs of 8.  A head dim that fills the
+  // form has one without bounds on its words: 258 us against 354 at 256, 105
+  // against 111 at 64, 77 against 97 at 96.
   if constexpr (kD < 256)
     if (group > 8)
       return dim == kD ? kernel_of<MmaEngine<T, kD, 2, true>>("mma x16") : kernel_of<MmaEngine<T, kD, 2, false>>("mma x16");
@@ -901,6 +909,9 @@ Kernel simt_kernel(int dim, int elements) {
   return kernel_of<SimtEngine<T, 1, 8, 32, kH>>("simt");
 }
 
+// Columns by the group: a smaller form has fewer sums per lane and more CTAs an SM
+// (32 bits; 2 columns against 8: head dim 64 with a window 32 against 53 us, 80 362
+// against 496, one head of 128 317 against 427; 4 against 8: 420 against 428).
 template <typename T>
 Kernel simt_kernel(int dim, int group, int elements) {
   return group <= 2   ? simt_kernel<T, 2>(dim, elements)
@@ -911,6 +922,8 @@ Kernel simt_kernel(int dim, int group, int elements) {
 // `align`: the power of two that divides every address and stride, in bytes.
 Kernel choose(int32_t dtype, int dim, int group, int align) {
   const int elements = align / akv_dtype_bytes(dtype);
+  // 16-bit rows of whole 16-byte words go to the tensor cores: head dim 80 in bf16,
+  // 4 query heads, 166 us against 824 for the 32-bit form.
   if (dtype == AKV_F32) return simt_kernel<float>(dim, group, elements);
   if (align >= 16) return dtype == AKV_F16 ? mma_kernel<__half>(dim, group) : mma_kernel<__nv_bfloat16>(dim, group);
   return dtype == AKV_F16 ? simt_kernel<__half>(dim, group, elements) : simt_kernel<__nv_bfloat16>(dim, group, elements);
