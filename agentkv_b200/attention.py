@@ -223,7 +223,8 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
     ``starts[-1]`` are padding and nothing is done for them.  Without it
     each row has one new token, row s of the operands (none where its length
     is 0).  No two rows may append to one block: make shared blocks
-    exclusive first (ensure_mutable_batch), as for kv_scatter.
+    exclusive first (ensure_mutable_batch), as for kv_scatter.  The operands do
+    not lie in the pool.
 
     ``rope`` (float32 [positions, rotary_dim], see rope_table) rotates the
     first rotary_dim dimensions of each new key by its position, pairs

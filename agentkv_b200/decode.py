@@ -12,8 +12,11 @@ uploaded) and per layer one ``append`` and one ``attend``:
         q = batch.append(layer, k, v, query=q, rope=rope)   # k, v: [64, kv_heads, head_dim]
         out = batch.attend(layer, q)                        # [64, heads, head_dim]
 
-The device tensors keep their addresses while the rows and the width do, so
-the calls of a step can be captured once and replayed after each ``advance``.
+The device tensors keep their addresses while the rows and the width do (give
+``width`` to hold it), so the calls of a step can be captured once and
+replayed after each ``advance``: a step captured after one of one token each
+serves such steps, one captured after an uneven one (operands with rows for
+the most tokens) any.
 """
 
 from __future__ import annotations
@@ -55,6 +58,8 @@ class DecodeBatch:
         self.tables = torch.zeros((self.rows, self.width), dtype=torch.int32, device=data.device)
         self.lengths = torch.zeros(self.rows, dtype=torch.int32, device=data.device)
         self.starts: Optional[torch.Tensor] = None  # of the last advance, when a row got more or less than one token
+        self._starts: Optional[torch.Tensor] = None  # where they lie, from the first such advance on
+        self._advanced = False  # the last advance's new tokens are there to be appended
         self._upload(ids)
         self.bounds: Optional[torch.Tensor] = None
         if bounds is not None and bounds is not False:
@@ -91,7 +96,9 @@ class DecodeBatch:
         if len(tokens) != len(self.handles):
             raise ValueError(f"DecodeBatch.advance: tokens for {len(tokens)} of {len(self.handles)} agents")
         pool, bs = self.pool, self.pool.block_size
+        self._advanced = False
         counts = [len(t) for t in tokens]
+        held = [len(pool.get_block_ids(h)) for h in self.handles]  # refuses a freed agent before anything changes
         if self._fixed:
             for h, n in zip(self.handles, counts):
                 if len(h.tokens) + n > self.width * bs:
@@ -106,9 +113,9 @@ class DecodeBatch:
             if first < shared:
                 raise RuntimeError("Cannot overwrite shared prefix blocks!")
             writes += [(h, b - shared) for b in range(first, last + 1)]
-        for h, n, new in zip(self.handles, counts, tokens):
+        for h, n, blocks in zip(self.handles, counts, held):
             if n:
-                required = (len(h.tokens) + n + bs - 1) // bs - len(pool.get_block_ids(h))
+                required = (len(h.tokens) + n + bs - 1) // bs - blocks
                 if required > 0:
                     pool.allocate_blocks(h, required)
         if writes:
@@ -117,20 +124,25 @@ class DecodeBatch:
             if n:
                 pool.append_tokens(h, list(new))
         self._upload([pool.get_block_ids(h) for h in self.handles])
-        if all(n == 1 for n in counts):
-            self.starts = None
-        else:
+        even = all(n == 1 for n in counts)
+        if not even and self._starts is None:
+            self._starts = torch.zeros(self.rows + 1, dtype=torch.int32, device=self.lengths.device)
+        if self._starts is not None:  # (kept right in even steps too: a captured uneven one reads them)
             starts = np.zeros(self.rows + 1, np.int32)
             starts[1 : len(counts) + 1] = np.cumsum(counts)
             starts[len(counts) + 1 :] = starts[len(counts)]
-            self.starts = torch.from_numpy(starts).to(self.lengths.device)
+            self._starts.copy_(torch.from_numpy(starts))
+        self.starts = None if even else self._starts
+        self._advanced = True
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, **kw) -> Optional[torch.Tensor]:
         """attention.kv_append of the last advance's new tokens, all agents'
         behind one another: key and value [tokens, kv_heads, head_dim] (where
         each agent got one token: of the agents, or of all rows, padding
         among them); ``query``, ``rope`` and the rest as there.  Returns the
-        rotated queries, if any."""
+        rotated queries, if any.  Refused before an advance and behind one that failed."""
+        if not self._advanced:
+            raise RuntimeError("DecodeBatch.append: no new tokens; advance() comes first")
         tables, lengths, n = self.tables, self.lengths, len(self.handles)
         if self.starts is None and key.shape[0] == n < self.rows:
             tables, lengths = tables[:n], lengths[:n]

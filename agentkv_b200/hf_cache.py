@@ -103,12 +103,13 @@ class AgentKVCache(DynamicCache):
         held = self._next_seen_tokens
         if n > held or self._table_dev is None:
             raise ValueError(f"AgentKVCache.attend: {n} queries over {held} tokens")
-        key = (held, n)
+        key, lens = (held, n), self._rows_len
         if self._rows_key != key:  # the same for every layer of a step
-            self._rows_len = torch.arange(held - n + 1, held + 1, dtype=torch.int32, device=query.device)
-            self._rows_key = key
+            lens = torch.arange(held - n + 1, held + 1, dtype=torch.int32, device=query.device)
+            if not (query.is_cuda and torch.cuda.is_current_stream_capturing()):  # made by the replay, not now
+                self._rows_key, self._rows_len = key, lens
         out = A.paged_attention(query[0].transpose(0, 1), self.pool._allocator._kv_data, layer_idx,
-                                self._table_dev.expand(n, -1), self._rows_len, scale=scale, window=window)
+                                self._table_dev.expand(n, -1), lens, scale=scale, window=window)
         return out.transpose(0, 1)[None]
 
     def _layer_done(self, layer_idx: int) -> None:

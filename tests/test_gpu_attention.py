@@ -673,3 +673,86 @@ def test_hf_cache_attends_in_place(dtype):
     assert ours.get_seq_length() == theirs.get_seq_length() == 29
     with pytest.raises(ValueError):
         ours.attend(torch.zeros(2, H * G, 1, D, dtype=t, device=DEV), 0)
+
+
+def _two_agents(**kw):
+    pool = AgentKVPool(config=PoolConfig(total_blocks=16, block_size=4, num_layers=1, num_kv_heads=1, head_dim=16,
+                                         dtype="float16", device="cuda"))
+    agents = [pool.create_root([]) for _ in range(2)]
+    return pool, agents, pool.decode_batch(agents, **kw)
+
+
+def test_append_needs_an_advance():
+    """Before one, or behind one that failed, there are no new tokens: the
+    agents' last ones must not be written over."""
+    x = torch.ones(2, 1, 16, dtype=F16, device=DEV)
+    _, _, batch = _two_agents()
+    with pytest.raises(RuntimeError, match="advance"):
+        batch.append(0, x, x)
+    batch.advance([[1], [2]])
+    batch.append(0, x, x, check=True)
+    with pytest.raises(MemoryError):
+        batch.advance([[1], [2] * 100])
+    with pytest.raises(RuntimeError, match="advance"):
+        batch.append(0, x, x)
+    batch.advance([[1], [2]])
+    batch.append(0, x, x, check=True)
+    assert torch.equal(batch.attend(0, x), x)
+
+
+def test_a_freed_agent_stops_an_advance_before_anything_changes():
+    pool, (a, b), batch = _two_agents()
+    batch.advance([[1], [2]])
+    pool.free(b)
+    with pytest.raises(Exception):
+        batch.advance([[1], []])
+    assert a.tokens == [1]
+
+
+def test_a_captured_uneven_step_follows_later_advances():
+    """The step's starts are at one address, and those of a later advance of
+    one token each are there too."""
+    def operands(x):
+        return torch.full((6, 1, 16), float(x), dtype=F16, device=DEV)
+
+    pool, agents, batch = _two_agents(width=4)
+    batch.advance([[1, 2], [3]])
+    k = operands(1)
+    batch.append(0, k, k, check=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        batch.append(0, k, k)
+    for turn, counts in enumerate(([0, 5], [1, 1], [3, 1])):
+        batch.advance([[7] * n for n in counts])
+        k.copy_(operands(turn + 2))
+        graph.replay()
+        torch.cuda.synchronize()
+    data = pool._allocator._kv_data
+    for agent, want in zip(agents, ([1, 1, 3, 4, 4, 4], [1, 2, 2, 2, 2, 2, 3, 4])):
+        ids = pool.get_block_ids(agent)
+        got = [data[ids[i // 4], 0, 0, 0, i % 4, 0].item() for i in range(len(agent.tokens))]
+        assert got == want
+
+
+def test_hf_cache_attends_eagerly_after_a_capture():
+    """The lengths that a captured call makes exist when it is replayed, not
+    before: an eager call makes its own."""
+    pool = AgentKVPool(config=PoolConfig(total_blocks=16, block_size=8, num_layers=1, num_kv_heads=1, head_dim=16,
+                                         dtype="float16", device="cuda"))
+    cache = AgentKVCache(pool, pool.create_root([]))
+    g = _gen(4)
+    k, v, q = (_randn(g, 1, 1, 5, 16, dtype=F16) for _ in range(3))
+    cache.store(k, v, 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        captured = cache.attend(q, 0)
+    eager = cache.attend(q, 0)
+    torch.cuda.synchronize()
+    x = q.double()[0, 0] @ k.double()[0, 0].T / 4
+    x = x.masked_fill(~torch.ones(5, 5, dtype=torch.bool, device=DEV).tril(), -math.inf)
+    _check(eager, (torch.softmax(x, 1) @ v.double()[0, 0])[None, None], F16)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(captured, eager)
