@@ -27,6 +27,8 @@ default one per device and stream, and one per device for captured calls;
 ``check=True`` waits and raises BlockOpError, which clears it).  The tokens
 concerned are left out; while the record holds an error, kv_append and
 key_bounds write nothing, as the framework's other writes (the reads go on).
+That starts with the call that reports it, so any of such a call's other tokens
+may be left out as well: append the batch again once the record is clear.
 Make a call once before capturing it (a pool's allocator does that for all).
 Forward only: an input that asks for a gradient is refused.
 """

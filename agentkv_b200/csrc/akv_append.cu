@@ -182,7 +182,10 @@ template <typename T, int kV>
 __global__ void __launch_bounds__(kThreads, 2) k_append(AppendParams p) {
   using Search = AkvRowSearch<kThreads>;
   __shared__ typename Search::Shared sh;
-  if (akv_failed(p.st)) return;
+  // One thread reads the record for all: CTAs of this launch write to it while
+  // others start, and a CTA whose warps saw different contents would search its
+  // row with the sums of warps that have left.
+  if (__syncthreads_or(threadIdx.x == 0 && akv_failed(p.st))) return;
   const int bl = p.kv.bs_log2;
   int32_t s;
   int64_t rest = 0;
@@ -203,6 +206,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_append(AppendParams p) {
     search.scan(sh, p.tab.rows, units);
     if (blockIdx.x >= search.total) return;
     search.find(sh, blockIdx.x, units, s, rest);
+    // (lengths or starts that are written to under the call can leave no such unit)
+    if (s < 0 || s >= p.tab.rows || rest < 0 || rest >= blocks_touched(p, s)) return;
   }
   const int32_t len = p.tab.lengths[s], n = new_tokens(p, s), old = len - n;
   const int32_t block = (old >> bl) + static_cast<int32_t>(rest);

@@ -712,7 +712,11 @@ typedef struct AkvHeads {
  *
  * No two rows may append to the same block in one call.  A block id out of
  * range, a position at or above rope_rows, or more new tokens than lengths
- * says are reported (AKV_ERR_OUT_OF_RANGE) and those tokens skipped. */
+ * says are reported (AKV_ERR_OUT_OF_RANGE) and those tokens skipped.  A call
+ * that reports one is not whole: CTAs that start behind the report do nothing, so any
+ * of its other tokens, or part of one's words, may be left unwritten too (each
+ * word that is written is right, and lies in its own block).  Append the
+ * batch again once the record is clear. */
 AKV_API int akv_kv_append(const AkvPagedPool* pool, const AkvPageBatch* batch, const AkvHeads* key,
                   const AkvHeads* value, int32_t n_tokens, const int32_t* starts, const float* rope,
                   int32_t rope_rows, int32_t rotary_dim, int32_t interleaved, const AkvHeads* query,
