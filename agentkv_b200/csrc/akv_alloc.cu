@@ -520,7 +520,9 @@ k_dec_small(AkvAllocState st, const int32_t* __restrict__ ids, int32_t n,
             int32_t* __restrict__ retired_out, AkvTick tk, AkvStatus* status) {
   __shared__ int ws[32];
   __shared__ DecPlan plan;
-  if (akv_failed(status)) return;  // nothing counted, nothing to clear
+  // (nothing counted, nothing to clear; one read for the CTA, since the first
+  // warps to count may already write to the record)
+  if (__syncthreads_or(threadIdx.x == 0 && akv_failed(status))) return;
   dec_count_body(st, ids, n, 0, 1, status);
   __syncthreads();
   const int n_ret = dec_flag_body(st, ids, 0, n, status, ws);
