@@ -38,6 +38,13 @@ constexpr float kLowest = -3.402823466e38f;
 // sums are the same for any m, so long as 2^(x - m) stays in range: at most
 // 2^8 here), which spares most steps the reduction over the lanes.
 constexpr float kLazy = 8.0f;
+// Weights as fp16 numbers: those have no step below 2^-24, so weights that are
+// to be in range must not lie near 1.  m is held kHalfBelow below the maximum and
+// raised once a score lies kHalfLazy above m: weights reach 2^15 at most (65,504 is
+// the largest number), the maximum's own is 2^11 at least, and what has no step
+// is under 2^-36 of it.
+constexpr float kHalfBelow = 11.0f;
+constexpr float kHalfLazy = 15.0f;
 constexpr int kLeast = 2;                  // chunks per CTA: a piece costs as much as one or two
 constexpr int kFan = 20;                   // pieces that are joined at a time
 constexpr int kMaxCtas = kFan * kFan * 2;  // two levels of joining
@@ -242,6 +249,9 @@ struct MmaEngine {
   static constexpr int kVi = kD / 64;      // the same of a value row,
   static constexpr bool kVr = kD % 64 != 0;  // and 8 bytes more
   static constexpr int kMt = kD / 16;      // output tiles of 16 dimensions
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
+  static constexpr float kBelow = kHalf ? kHalfBelow : 0.f;  // m lies this far below the maximum at most
+  static constexpr float kRaise = kHalf ? kHalfLazy : kLazy;
 
   uint4 q[kN][kKi];
   uint4 ka[kKi], kb[kKi];
@@ -384,16 +394,17 @@ struct MmaEngine {
           }
       };
       exponents();
-      if (__any_sync(kFullWarp, above > kLazy)) {
+      if (__any_sync(kFullWarp, above > kRaise)) {
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float top = m[n][x];
+            float top = m[n][x] + kBelow;
             if (now >> g & 1) top = fmaxf(top, sc[n][x] * p.scale_log2);
             if (now >> (g + 8) & 1) top = fmaxf(top, sc[n][x + 2] * p.scale_log2);
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullWarp, top, off));
+            top -= kBelow;
             const float by = exp2_fast(m[n][x] - top);
             m[n][x] = top;
             l[n][x] *= by;
@@ -407,7 +418,9 @@ struct MmaEngine {
       }
       // The weights go into the product as the sum of two 16-bit numbers:
       // one alone would be off by half a step of the type, as much as the
-      // output's own rounding; the time is the memory's either way.
+      // output's own rounding; the time is the memory's either way.  The two
+      // are off by 2^-18 of the weight in bf16; in fp16 by 2^-24 of it and, where the
+      // second is below the type's normal range, by 2^-25 (2^-36 of the largest weight).
       uint32_t hi[kN][2], lo[kN][2];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {

@@ -101,3 +101,70 @@ def test_ragged_append_with_bad_rows_writes_right_words_or_none(kind):
     A.kv_append(pool, 0, k, v, good_table, lens, starts=starts, rope=good_rope, query=q, query_out=qo, bounds=bounds,
                 check=True)
     assert torch.equal(pool, right) and torch.equal(bounds, rb) and torch.equal(qo, rq)
+
+
+# ── attention: one score far above very many others ──────────────────────────
+@pytest.mark.parametrize("gap", [0.0, 8.0, 10.0, 13.0, 15.0, 17.0, 17.5, 18.0, 20.0])
+@pytest.mark.parametrize("dtype,G,D", [(F16, 4, 128), (F16, 9, 64), (F16, 4, 256), (F16, 2, 80), (F16, 1, 96), (BF16, 4, 128),
+                                       (F32, 2, 64)])
+def test_small_weights_count_beside_a_large_one(dtype, G, D, gap):
+    """The first key scores `gap` above all the others and its value is 0, as
+    a model's first token often has it: the output is the others' share.
+
+    With w_j = e^(x_j - max), of which the two 16-bit numbers of a weight leave out
+    2^-18 w_j + 2^-36 (bf16: no second part) and 32-bit scores and the hardware's exp2
+    1e-5 w_j (as derived for the plain cases), |error| <= u |o| +
+    (2e-5 sum w |v| + 2^-36 sum |v|) / sum w.  An output below the type's normal range
+    is off by half its smallest step."""
+    n, H, bs = 100_001, 2, 16
+    g = _gen(int(gap * 10) + D)
+    blocks = -(-n // bs)
+    pool = torch.zeros((blocks, 1, 2, H, bs, D), dtype=dtype, device=DEV)
+    pool[:, 0, 1] = (1 + 0.5 * _randn(g, blocks, H, bs, D, dtype=F32)).to(dtype)
+    pool[0, 0, 1, :, 0] = 0
+    q = _randn(g, 1, H * G, D, dtype=F32).sign().to(dtype)  # of +-1: all the heads' scores at one gap
+    q = q.view(H, G, D)[:, :1].expand(H, G, D).reshape(1, H * G, D).contiguous()
+    pool[0, 0, 0, :, 0] = (q.view(H, G, D)[:, 0].float() * (gap / D)).to(dtype)
+    table = torch.arange(blocks, dtype=torch.int32, device=DEV)[None]
+    out, lse = A.paged_attention(q, pool, 0, table, torch.tensor([n], dtype=torch.int32, device=DEV), scale=1.0,
+                                 return_lse=True, check=True)
+    k, v = (pool[:, 0, i].double().permute(1, 0, 2, 3).reshape(H, 1, -1, D)[:, :, :n] for i in range(2))
+    x = q.view(H, G, 1, D).double() @ k.transpose(2, 3)
+    w = torch.exp(x - x.amax(3, keepdim=True))
+    total = w.sum(3, keepdim=True)
+    want = (w @ v / total).view(1, H * G, D)
+    u = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * u
+    allowed = (2e-5 * (w @ v.abs()) + 2.0 ** -36 * v.abs().sum(2, keepdim=True)) / total
+    err = (out.double() - want).abs()
+    assert (err <= u * want.abs() + tiny + allowed.view(1, H * G, D)).all(), (err / want.abs()).max().item()
+    assert ((lse.double() - torch.logsumexp(x, 3).view(1, -1)).abs() <= 1e-4).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_fp16_scores_that_rise_step_by_step(D):
+    """Scores that rise by less than what makes the running maximum move, then by
+    more, over a range far wider than fp16's: no weight passes the largest fp16 number."""
+    n, H, G, bs = 4_000, 1, 8, 16
+    g = _gen(D)
+    blocks = -(-n // bs)
+    pool = _randn(g, blocks, 1, 2, H, bs, D, dtype=F16)
+    rise = torch.linspace(-60, 60, blocks * bs, device=DEV)
+    for order in (rise, rise.flip(0), rise[torch.randperm(rise.numel(), generator=g, device=DEV)]):
+        pool[:, 0, 0] = 0
+        pool[:, 0, 0, 0, :, 0] = order.view(blocks, bs).to(F16)
+        q = torch.zeros(1, G, D, dtype=F16, device=DEV)
+        q[0, :, 0] = torch.tensor([1.0, 0.5, 0.25, 2.0, -1.0, -0.5, 4.0, 0.0])
+        table = torch.arange(blocks, dtype=torch.int32, device=DEV)[None]
+        out, lse = A.paged_attention(q, pool, 0, table, torch.tensor([n], dtype=torch.int32, device=DEV), scale=1.0,
+                                     return_lse=True, check=True)
+        k, v = (pool[:, 0, i, 0].double().reshape(-1, D)[:n] for i in range(2))
+        x = q[0].double() @ k.T
+        w = torch.softmax(x, 1)
+        want = w @ v
+        err = (out[0].double() - want).abs()
+        # scores up to 240 in 32 bits, scaled to base 2 and taken off one another: off by 3 * 2^-24 * 347 = 6e-5
+        # of the weight each, with the rest as above
+        allowed = 2.0 ** -11 * want.abs() + 1e-4 * (w @ v.abs()) + 2.0 ** -25
+        assert (err <= allowed).all(), (err - allowed).max().item()
+        assert ((lse[0].double() - torch.logsumexp(x, 1)).abs() <= 1e-3).all()
