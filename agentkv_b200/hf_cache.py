@@ -58,8 +58,10 @@ class AgentKVCache(DynamicCache):
         self.key_cache = []
         self.value_cache = []
         self._table: Optional[list] = None
+        self._table_buf: Optional[torch.Tensor] = None  # _table_dev's memory, written in place while it has room
         self._table_dev: Optional[torch.Tensor] = None
-        self._table_version = 0  # bumped whenever _table_dev is replaced
+        self._captured: list = []  # the buffers that captured calls read: kept, and kept up to date
+        self._table_version = 0  # bumped whenever _table_dev changes
         self._slots_key: Optional[tuple] = None  # (first new token, count, table version) of _slots_dev
         self._slots_dev: Optional[torch.Tensor] = None
         self._rows_key: Optional[tuple] = None  # (tokens held, queries) of _rows_len
@@ -71,7 +73,14 @@ class AgentKVCache(DynamicCache):
     def _device_table(self, ids: list) -> torch.Tensor:
         if self._table != ids:
             self._table = list(ids)
-            self._table_dev = torch.tensor(ids, dtype=torch.int32).to(self.pool._allocator._kv_data.device)
+            host, n = torch.tensor(ids, dtype=torch.int32), len(ids)
+            if self._table_buf is None or n > self._table_buf.numel():
+                self._table_buf = torch.zeros(max(16, 2 * n), dtype=torch.int32,
+                                              device=self.pool._allocator._kv_data.device)
+            for buf in [b for b in self._captured if b is not self._table_buf] + [self._table_buf]:
+                m = min(n, buf.numel())
+                buf[:m].copy_(host[:m])
+            self._table_dev = self._table_buf[:n]
             self._table_version += 1
         return self._table_dev
 
@@ -89,14 +98,20 @@ class AgentKVCache(DynamicCache):
     def store(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
         """update() without assembling the layer's K and V: for a model that
         reads them where they lie, with attend() (called after store(), for
-        each layer)."""
+        each layer).  Not while capturing: a replay would write this step's
+        places, whose blocks may have become another agent's."""
+        if A._capturing():
+            raise RuntimeError("AgentKVCache.store: not while capturing (DecodeBatch.append can be captured)")
         self._write(key_states, value_states, layer_idx)
         self._layer_done(layer_idx)
 
     def attend(self, query: torch.Tensor, layer_idx: int, *, scale: Optional[float] = None,
                window: int = 0) -> torch.Tensor:
         """Causal attention of the last update's (or store's) n new tokens,
-        query [1, heads, n, head_dim] to the same shape, over the layer's blocks."""
+        query [1, heads, n, head_dim] to the same shape, over the layer's blocks.
+        A captured call attends over as many tokens as at its capture in every
+        replay, in the blocks that hold them by then; the cache has to be kept
+        as long as the graph."""
         if query.dim() != 4 or query.shape[0] != 1:
             raise ValueError("AgentKVCache requires batch_size=1")
         n = query.shape[2]
@@ -104,10 +119,14 @@ class AgentKVCache(DynamicCache):
         if n > held or self._table_dev is None:
             raise ValueError(f"AgentKVCache.attend: {n} queries over {held} tokens")
         key, lens = (held, n), self._rows_len
-        if self._rows_key != key:  # the same for every layer of a step
+        capturing = query.is_cuda and A._capturing()
+        if capturing or self._rows_key != key:  # the same for every layer of a step
+            # (while capturing: made by the graph, in memory of its own)
             lens = torch.arange(held - n + 1, held + 1, dtype=torch.int32, device=query.device)
-            if not (query.is_cuda and torch.cuda.is_current_stream_capturing()):  # made by the replay, not now
+            if not capturing:
                 self._rows_key, self._rows_len = key, lens
+        if capturing and not any(b is self._table_buf for b in self._captured):
+            self._captured.append(self._table_buf)
         out = A.paged_attention(query[0].transpose(0, 1), self.pool._allocator._kv_data, layer_idx,
                                 self._table_dev.expand(n, -1), lens, scale=scale, window=window)
         return out.transpose(0, 1)[None]

@@ -11,6 +11,7 @@ from agentkv_b200 import AgentKVPool, PoolConfig
 from agentkv_b200 import _native as N
 from agentkv_b200 import attention as A
 from agentkv_b200 import kernels as K
+from agentkv_b200.hf_cache import AgentKVCache
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +169,72 @@ def test_fp16_scores_that_rise_step_by_step(D):
         allowed = 2.0 ** -11 * want.abs() + 1e-4 * (w @ v.abs()) + 2.0 ** -25
         assert (err <= allowed).all(), (err - allowed).max().item()
         assert ((lse[0].double() - torch.logsumexp(x, 1)).abs() <= 1e-3).all()
+
+
+# ── AgentKVCache.attend, captured ────────────────────────────────────────────
+def _one_head_cache(total=64, bs=8):
+    pool = AgentKVPool(config=PoolConfig(total_blocks=total, block_size=bs, num_layers=1, num_kv_heads=1, head_dim=16,
+                                         dtype="float16", device="cuda"))
+    return pool, AgentKVCache(pool, pool.create_root([]))
+
+
+def _capture(call):
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        out = call()
+    return graph, out
+
+
+def test_a_captured_cache_attention_outlives_later_steps():
+    """Eager call, capture of the same call, later steps with other lengths and
+    more blocks, and memory asked for again in between: the replay still
+    attends over the tokens of its capture."""
+    pool, cache = _one_head_cache()
+    g = _gen(6)
+    k, v, q = (_randn(g, 1, 1, 5, 16, dtype=F16) for _ in range(3))
+    cache.store(k, v, 0)
+    want = cache.attend(q, 0).clone()
+    graph, got = _capture(lambda: cache.attend(q, 0))
+    taken = []
+    for n in (1, 30, 1, 200):  # past the table's room
+        x, y = (_randn(g, 1, 1, n, 16, dtype=F16) for _ in range(2))
+        cache.store(x, y, 0)
+        cache.attend(y, 0)
+        torch.cuda.synchronize()
+        for size in range(1, 65):  # what was let go is handed out again, with contents that are no length or block
+            taken.append(torch.full((size,), 2 ** 30 + 7, dtype=torch.int32, device=DEV))
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), n
+    assert K.read_status(pool._allocator._status)[0] == 0
+
+
+def test_a_captured_cache_attention_follows_a_copied_block():
+    """The tokens' last block is shared by a fork and copied when the agent
+    goes on: the replay reads the agent's own, whatever the fork's becomes."""
+    pool, cache = _one_head_cache()
+    g = _gen(7)
+    k, v, q = (_randn(g, 1, 1, 5, 16, dtype=F16) for _ in range(3))
+    cache.store(k, v, 0)
+    want = cache.attend(q, 0).clone()
+    graph, got = _capture(lambda: cache.attend(q, 0))
+    old = pool.get_block_ids(cache.handle)
+    child = cache.fork()
+    cache.store(k[:, :, :1], v[:, :, :1], 0)
+    assert pool.get_block_ids(cache.handle) != old == pool.get_block_ids(child.handle)
+    pool._allocator._kv_data[old[0]] = math.nan
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_a_cache_refuses_to_store_while_capturing():
+    pool, cache = _one_head_cache()
+    k = torch.ones(1, 1, 5, 16, dtype=F16, device=DEV)
+    with pytest.raises(RuntimeError, match="capturing"):
+        _capture(lambda: (k + 1, cache.store(k, k, 0)))
+    torch.cuda.synchronize()
+    cache.store(k, k, 0)
+    assert torch.equal(cache.attend(k, 0), k)
