@@ -150,6 +150,23 @@ def _span(x: torch.Tensor) -> tuple:
     return x.data_ptr(), x.data_ptr() + size * x.element_size()
 
 
+def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether no element of y shares memory with one of x: their addresses
+    do not meet, or do not modulo one of x's strides (views of one buffer
+    next to one another in each of its rows, as of a fused projection)."""
+    (a, b), (c, d) = _span(x), _span(y)
+    if a >= d or c >= b:
+        return True
+    for period in {n * x.element_size() for n in x.stride() if n > 0}:
+        # dimensions whose steps are whole periods stay at one place in it
+        ex, ey = (t.element_size() + sum((n - 1) * s * t.element_size() for n, s in zip(t.shape, t.stride())
+                                         if n > 1 and s * t.element_size() % period) for t in (x, y))
+        at = (c - a) % period
+        if at >= ex and at + ey <= period:
+            return True
+    return False
+
+
 def _check_output(out: torch.Tensor, like: torch.Tensor, name: str, what: str, *inputs: torch.Tensor) -> None:
     """out has like's shape, no two elements of it share memory, and none
     of it lies within an input."""
@@ -161,10 +178,8 @@ def _check_output(out: torch.Tensor, like: torch.Tensor, name: str, what: str, *
             if n > 1 and s < span:
                 raise ValueError(f"{what}: {name}'s elements overlap")
             span += (n - 1) * s
-    a, b = _span(out)
     for x in inputs:
-        c, d = _span(x)
-        if a < d and c < b:
+        if not _apart(out, x):
             raise ValueError(f"{what}: {name} shares memory with an input")
 
 

@@ -1,0 +1,57 @@
+"""Which tensors attention's operators take as outputs beside their inputs:
+views of one buffer that share no element are apart, others are not."""
+
+import itertools
+import random
+
+import pytest
+import torch
+
+from agentkv_b200 import attention as A
+
+
+def _addresses(x):
+    at = torch.zeros(1, dtype=torch.int64)
+    for n, s in zip(x.shape, x.stride()):
+        at = (at[:, None] + torch.arange(n) * s).reshape(-1)
+    return {x.data_ptr() + int(i) * x.element_size() + b for i in at for b in range(x.element_size())}
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 5])
+def test_views_of_a_fused_projection_are_apart(tokens):
+    Hq, H, D = 6, 2, 8
+    packed = torch.zeros(tokens, Hq + 2 * H, D, dtype=torch.bfloat16)       # [tokens, all heads, head_dim]
+    q, k, v = packed[:, :Hq], packed[:, Hq:Hq + H], packed[:, Hq + H:]
+    third = torch.zeros(tokens, 3, H, D, dtype=torch.float16).unbind(1)       # [tokens, (q, k, v), heads, head_dim]
+    by_head = torch.zeros(tokens, H, 3, D, dtype=torch.float32).unbind(2)     # [tokens, heads, (q, k, v), head_dim]
+    by_dim = torch.zeros(tokens, H, 3 * D, dtype=torch.float32).split(D, 2)   # [tokens, heads, (q, k, v) of head_dim]
+    heads_first = torch.zeros(3, H, tokens, D).transpose(1, 2).unbind(0)      # (q, k, v) of [heads, tokens, head_dim]
+    for views in ((q, k, v), third, by_head, by_dim, heads_first):
+        for x, y in itertools.permutations(views, 2):
+            assert A._apart(x, y)
+            A._check_output(x, x, "query_out", "kv_append", y)
+    for x, y in ((q, packed[:, Hq - 1:Hq + 1]), (k, packed[:, :Hq + 1]), (v, packed), (packed, v), (q, q)):
+        assert not A._apart(x, y)
+        with pytest.raises(ValueError, match="shares memory"):
+            A._check_output(x, x, "query_out", "kv_append", y)
+
+
+def test_no_overlap_is_missed():
+    """Random views of one buffer against their elements' addresses: what is
+    called apart has none in common."""
+    rng = random.Random(5)
+    buf = torch.zeros(4000, dtype=torch.float16)
+    called = met = 0
+    for _ in range(4000):
+        views = []
+        for _ in range(2):
+            shape = [rng.randint(1, 5), rng.randint(1, 4), rng.choice([1, 2, 3, 4])]
+            stride = [rng.choice([0, 4, 8, 12, 16, 24, 30]), rng.choice([0, 2, 4, 8, 16]), 1]
+            x = buf[rng.randint(0, 60):].as_strided(shape, stride, rng.randint(0, 60))
+            views.append(x.view(torch.bfloat16) if rng.random() < 0.3 else x)
+        common = bool(_addresses(views[0]) & _addresses(views[1]))
+        apart = A._apart(*views)
+        assert not (apart and common), [(x.shape, x.stride(), x.storage_offset()) for x in views]
+        called += apart
+        met += not common
+    assert called > 0.6 * met  # and it is not all refused

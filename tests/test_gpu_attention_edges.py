@@ -238,3 +238,30 @@ def test_a_cache_refuses_to_store_while_capturing():
     torch.cuda.synchronize()
     cache.store(k, k, 0)
     assert torch.equal(cache.attend(k, 0), k)
+
+
+# ── append on views of one fused projection ──────────────────────────────────
+@pytest.mark.parametrize("layout", ["heads", "thirds", "by head"])
+def test_append_turns_a_fused_projection_in_place(layout):
+    """query, key and value as views of one buffer and the rotated queries over
+    the queries: as with memory of their own, and keys and values untouched."""
+    H, D, bs, rows, T = 2, 64, 8, 3, 9
+    g = _gen(12)
+    if layout == "heads":
+        packed = _randn(g, T, 4 * H, D, dtype=BF16)
+        q, k, v = packed[:, :2 * H], packed[:, 2 * H:3 * H], packed[:, 3 * H:]
+    elif layout == "thirds":
+        packed = _randn(g, T, 3, H, D, dtype=BF16)
+        q, k, v = packed.unbind(1)
+    else:
+        packed = _randn(g, T, H, 3 * D, dtype=BF16)
+        q, k, v = packed.split(D, 2)
+    pools = [torch.zeros((9, 1, 2, H, bs, D), dtype=BF16, device=DEV) for _ in range(2)]
+    table = torch.arange(9, dtype=torch.int32, device=DEV).view(rows, 3)
+    lengths = torch.tensor([11, 4, 20], dtype=torch.int32, device=DEV)
+    kw = dict(starts=[0, 5, 6, 9], rope=A.rope_table(D, 32, device=DEV), check=True)
+    want = A.kv_append(pools[0], 0, k.contiguous(), v.contiguous(), table, lengths, query=q.contiguous(), **kw)
+    before = k.clone(), v.clone()
+    got = A.kv_append(pools[1], 0, k, v, table, lengths, query=q, query_out=q, **kw)
+    assert got is q and torch.equal(q, want) and torch.equal(pools[0], pools[1])
+    assert torch.equal(k, before[0]) and torch.equal(v, before[1])
