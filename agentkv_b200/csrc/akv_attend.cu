@@ -1012,7 +1012,7 @@ int akv_attend_prepare() {
   for (int32_t dtype : {AKV_F32, AKV_F16, AKV_BF16})
     for (int group : {1, 4, 8, 9})
       for (int dim : {56, 64, 80, 96, 104, 128, 200, 256})
-        for (int align : {4, 16}) {
+        for (int align : {4, 8, 16}) {
           const Kernel k = choose(dtype, dim, group, align);
           if (int rc = akv_load_kernel(reinterpret_cast<const void*>(k.attend), k.name)) return rc;
         }
@@ -1030,7 +1030,7 @@ extern "C" int64_t akv_paged_attention_scratch_bytes(const AkvPagedPool* pool, i
   const int64_t chunks = chunks_of(pool->block_size, table_width, keep);
   if (rows == 0) return 0;
   int64_t most = 0;
-  for (int align : {4, 16}) {  // whichever engine the addresses will allow
+  for (int align : {4, 8, 16}) {  // whichever engine the addresses will allow
     const Kernel k = choose(pool->dtype, kv.dim, group, align);
     const int64_t pairs = static_cast<int64_t>(kv.heads) * parts_of(k, group);
     const int64_t n = scratch_of(k, grid_of(k, rows, pairs, chunks), kv.dim);

@@ -7,6 +7,7 @@ import random
 import pytest
 import torch
 
+from agentkv_b200 import _native as N
 from agentkv_b200 import attention as A
 
 
@@ -55,3 +56,23 @@ def test_no_overlap_is_missed():
         called += apart
         met += not common
     assert called > 0.6 * met  # and it is not all refused
+
+
+@pytest.mark.parametrize("dtype", [N.F32, N.F16, N.BF16])
+def test_the_work_space_is_enough_for_every_alignment(dtype):
+    """The size does not depend on the addresses, the engine does: a call of exactly that
+    size is refused for its missing counters alone."""
+    rng = random.Random(dtype)
+    size = 4 if dtype == N.F32 else 2
+    for dim in [1, 2, 4, 7, 8, 12, 56, 60, 64, 68, 72, 80, 96, 100, 104, 128, 130, 132, 136, 200, 204, 252, 256]:
+        for group in [1, 2, 3, 4, 5, 8, 9, 16, 17]:
+            rows, width, keep, bs = rng.choice([1, 3, 200]), rng.choice([1, 7, 500]), rng.choice([0, 2]), 16
+            geometry = (64, 2, 2, bs, dim, dtype, 0, 0)
+            need = N.lib.akv_paged_attention_scratch_bytes(A._POOL(0, *geometry), rows, width, group, keep)
+            assert need > 0
+            for at in (1 << 20, (1 << 20) + 8, (1 << 20) + 4, (1 << 20) + size):
+                heads = A._HEADS(at, 2 * group * dim, dim)
+                batch = A._BATCH(1 << 20, 1 << 20, width, width, rows)
+                rc = N.lib.akv_paged_attention(A._POOL(1 << 20, *geometry), batch, heads, group, 1.0, 0,
+                                               1 << 20 if keep else None, keep, heads, None, 1 << 20, need, None, None, None)
+                assert rc == N.AKV_ERR_INVALID_ARG and "counters" in N.last_error(), (dim, group, at, N.last_error())

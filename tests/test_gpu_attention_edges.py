@@ -3,6 +3,8 @@ batches with bad rows, scores far apart, agents on a matched prefix, captured
 calls whose inputs move on."""
 
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -265,3 +267,35 @@ def test_append_turns_a_fused_projection_in_place(layout):
     got = A.kv_append(pools[1], 0, k, v, table, lengths, query=q, query_out=q, **kw)
     assert got is q and torch.equal(q, want) and torch.equal(pools[0], pools[1])
     assert torch.equal(k, before[0]) and torch.equal(v, before[1])
+
+
+# ── first launches ───────────────────────────────────────────────────────────
+_FIRST = '''
+import torch
+from agentkv_b200 import AgentKVPool, PoolConfig, attention as A
+dev = torch.device("cuda", 0)
+AgentKVPool(config=PoolConfig(total_blocks=4, block_size=16, num_layers=1, num_kv_heads=1, head_dim=64,
+                              dtype="float16", device="cuda"))
+forms = []
+for dtype in (torch.float16, torch.bfloat16, torch.float32):
+    for D, group in ((12, 1), (12, 4), (12, 5), (100, 2), (100, 3), (100, 8), (204, 1), (204, 4), (204, 7), (7, 1), (130, 9)):
+        pool = torch.ones((3, 1, 2, 1, 16, D), dtype=dtype, device=dev)
+        forms.append((torch.ones((1, group, D), dtype=dtype, device=dev), pool))
+table = torch.tensor([[2, 0]], dtype=torch.int32, device=dev)
+lengths = torch.tensor([20], dtype=torch.int32, device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, capture_error_mode="global"):
+    outs = [A.paged_attention(q, pool, 0, table, lengths) for q, pool in forms]
+graph.replay()
+torch.cuda.synchronize()
+assert all((o == 1).all() for o in outs)
+print("right")
+'''
+
+
+def test_first_launches_of_every_form_inside_a_capture():
+    """A pool's making loads the kernels: head dims and alignments of every
+    form can be captured without an eager call of theirs before."""
+    r = subprocess.run([sys.executable, "-c", _FIRST], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "right" in r.stdout, r.stderr[-2000:]
