@@ -26,7 +26,9 @@ from typing import List, Optional, Sequence
 import numpy as np
 import torch
 
+from . import _native as N
 from . import attention as A
+from . import kernels as K
 from .radix_tree import NodeHandle
 
 
@@ -37,7 +39,12 @@ class DecodeBatch:
     needed when None).  With ``bounds`` (True, or a tensor that several
     batches of the pool share; see attention.key_bounds) ``append`` keeps the
     blocks' key bounds, which ``attend(keep=...)`` ranks them by; a new tensor
-    starts with the bounds of the blocks that the agents hold."""
+    starts with the bounds of the blocks that the agents hold.
+
+    What only the device can see goes to the batch's own record, ``status``
+    (captured calls' too): ``check()`` waits for it and raises, and ``advance``
+    raises, before anything changes, what has come back by then of earlier steps
+    (whose appends from the refused one on have written nothing)."""
 
     def __init__(self, pool, handles: Sequence[NodeHandle], *, rows: Optional[int] = None, width: Optional[int] = None,
                  bounds=None) -> None:
@@ -60,6 +67,9 @@ class DecodeBatch:
         self.starts: Optional[torch.Tensor] = None  # of the last advance, when a row got more or less than one token
         self._starts: Optional[torch.Tensor] = None  # where they lie, from the first such advance on
         self._advanced = False  # the last advance's new tokens are there to be appended
+        self._positions = 0  # what the longest row that got new tokens holds
+        self.status = torch.zeros(N.STATUS_BYTES // 4, dtype=torch.int32, device=data.device)
+        self._seen = torch.zeros(N.STATUS_BYTES // 4, dtype=torch.int32, pin_memory=data.is_cuda)
         self._upload(ids)
         self.bounds: Optional[torch.Tensor] = None
         if bounds is not None and bounds is not False:
@@ -67,7 +77,7 @@ class DecodeBatch:
                 n_blocks, layers, _, heads, _, dim = data.shape
                 self.bounds = torch.zeros((n_blocks, layers, heads, 2, dim), dtype=data.dtype, device=data.device)
                 for layer in range(layers):
-                    A.key_bounds(data, layer, self.tables, self.lengths, self.bounds)
+                    A.key_bounds(data, layer, self.tables, self.lengths, self.bounds, status=self.status)
             else:
                 A._check_bounds(bounds, data, "DecodeBatch")
                 self.bounds = bounds
@@ -88,6 +98,13 @@ class DecodeBatch:
         self.tables.copy_(torch.from_numpy(table))
         self.lengths.copy_(torch.from_numpy(lens))
 
+    def check(self) -> None:
+        """Wait for the calls so far and raise BlockOpError for the first that
+        the device refused, if any (which clears it)."""
+        self._seen.zero_()
+        if self.status.is_cuda:
+            K.raise_for_status(self.status)
+
     def advance(self, tokens: Sequence[Sequence[int]]) -> None:
         """Give agent i the new tokens ``tokens[i]`` (none: it sits this step
         out): room is allocated, blocks that the new tokens go to are made
@@ -97,6 +114,8 @@ class DecodeBatch:
             raise ValueError(f"DecodeBatch.advance: tokens for {len(tokens)} of {len(self.handles)} agents")
         pool, bs = self.pool, self.pool.block_size
         self._advanced = False
+        if self._seen[0]:
+            self.check()
         counts = [len(t) for t in tokens]
         held = [len(pool.get_block_ids(h)) for h in self.handles]  # refuses a freed agent before anything changes
         if self._fixed:
@@ -133,6 +152,9 @@ class DecodeBatch:
             starts[len(counts) + 1 :] = starts[len(counts)]
             self._starts.copy_(torch.from_numpy(starts))
         self.starts = None if even else self._starts
+        self._positions = max([len(h.tokens) for h, n in zip(self.handles, counts) if n], default=0)
+        if self.status.is_cuda:
+            self._seen.copy_(self.status, non_blocking=True)
         self._advanced = True
 
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, **kw) -> Optional[torch.Tensor]:
@@ -143,6 +165,10 @@ class DecodeBatch:
         rotated queries, if any.  Refused before an advance and behind one that failed."""
         if not self._advanced:
             raise RuntimeError("DecodeBatch.append: no new tokens; advance() comes first")
+        rope = kw.get("rope")
+        if rope is not None and rope.shape[0] < self._positions:
+            raise ValueError(f"DecodeBatch.append: a rope table of {rope.shape[0]} positions for {self._positions} tokens")
+        kw.setdefault("status", self.status)
         tables, lengths, n = self.tables, self.lengths, len(self.handles)
         if self.starts is None and key.shape[0] == n < self.rows:
             tables, lengths = tables[:n], lengths[:n]
@@ -152,10 +178,11 @@ class DecodeBatch:
         """attention.paged_attention of one query per row, [rows, heads,
         head_dim], over the row's tokens; with ``keep`` over the `keep` blocks
         that attention.select_blocks picks (needs the batch's bounds)."""
+        kw.setdefault("status", self.status)
         if keep:
             if self.bounds is None:
                 raise ValueError("DecodeBatch.attend: keep needs a batch with bounds")
             kw["selected"] = A.select_blocks(query, self.bounds, layer, self.tables, self.lengths, keep,
                                              block_size=self.pool.block_size, first=first, last=last,
-                                             status=kw.get("status"))
+                                             status=kw["status"])
         return A.paged_attention(query, self._data, layer, self.tables, self.lengths, **kw)

@@ -128,7 +128,8 @@ class AgentKVCache(DynamicCache):
         if capturing and not any(b is self._table_buf for b in self._captured):
             self._captured.append(self._table_buf)
         out = A.paged_attention(query[0].transpose(0, 1), self.pool._allocator._kv_data, layer_idx,
-                                self._table_dev.expand(n, -1), lens, scale=scale, window=window)
+                                self._table_dev.expand(n, -1), lens, scale=scale, window=window,
+                                status=self.pool._allocator._status)
         return out.transpose(0, 1)[None]
 
     def _layer_done(self, layer_idx: int) -> None:

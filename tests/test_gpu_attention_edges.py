@@ -299,3 +299,72 @@ def test_first_launches_of_every_form_inside_a_capture():
     form can be captured without an eager call of theirs before."""
     r = subprocess.run([sys.executable, "-c", _FIRST], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "right" in r.stdout, r.stderr[-2000:]
+
+
+# ── DecodeBatch: errors come back ────────────────────────────────────────────
+def _batch(agents=2, bs=4, D=16, **kw):
+    pool = AgentKVPool(config=PoolConfig(total_blocks=64, block_size=bs, num_layers=1, num_kv_heads=1, head_dim=D,
+                                         dtype="float16", device="cuda"))
+    handles = [pool.create_root([]) for _ in range(agents)]
+    return pool, handles, pool.decode_batch(handles, **kw)
+
+
+def test_a_rope_table_that_is_too_short_is_refused_on_the_host():
+    pool, _, batch = _batch()
+    x = torch.ones(2, 1, 16, dtype=F16, device=DEV)
+    batch.advance([[1] * 6, [2]])
+    k = torch.ones(7, 1, 16, dtype=F16, device=DEV)
+    with pytest.raises(ValueError, match="rope table of 5 positions for 6 tokens"):
+        batch.append(0, k, k, rope=A.rope_table(16, 5, device=DEV))
+    batch.append(0, k, k, rope=A.rope_table(16, 6, device=DEV))
+    batch.advance([[], [3]])  # the long row sits this one out: its positions are not turned
+    batch.append(0, x[:1], x[:1], rope=A.rope_table(16, 5, device=DEV))
+    batch.check()
+
+
+def test_what_a_captured_step_reports_is_raised_by_a_later_advance():
+    """A captured append whose rope table the rows outgrow: the next advances
+    raise it, before anything changes, and the batch goes on once it is clear."""
+    pool, (a, b), batch = _batch(width=4)
+    x = torch.ones(2, 1, 16, dtype=F16, device=DEV)
+    rope = A.rope_table(16, 3, device=DEV)
+    batch.advance([[1], [2]])
+    batch.append(0, x, x, rope=rope, check=True)
+    graph, _ = _capture(lambda: batch.append(0, x, x, rope=rope))
+    with pytest.raises(K.BlockOpError):
+        for _ in range(6):
+            batch.advance([[1], [2]])
+            graph.replay()
+            torch.cuda.synchronize()
+    held = len(a.tokens)
+    assert held in (4, 5) and len(b.tokens) == held
+    batch.check()  # cleared
+    batch.advance([[1], [2]])
+    assert len(a.tokens) == held + 1
+    batch.append(0, x, x)
+    batch.check()
+    graph.replay()
+    with pytest.raises(K.BlockOpError):
+        batch.check()
+    batch.check()
+
+
+def test_what_attend_reports_is_the_batch_s_own():
+    """Not the allocator's record, behind which its own calls would stop."""
+    pool, _, batch = _batch(bounds=True)
+    x = torch.ones(2, 1, 16, dtype=F16, device=DEV)
+    batch.advance([[1] * 9, [2] * 9])
+    k = torch.ones(18, 1, 16, dtype=F16, device=DEV)
+    batch.append(0, k, k)
+    batch.check()
+    batch.tables[0, 1] = 64
+    batch.attend(0, x)
+    with pytest.raises(K.BlockOpError):
+        batch.check()
+    batch.attend(0, x, keep=2)
+    with pytest.raises(K.BlockOpError):
+        batch.check()
+    pool._allocator.check()
+    batch.advance([[1], [2]])  # the tables are made anew
+    batch.append(0, x, x)
+    assert torch.equal(batch.attend(0, x, check=True), x)
