@@ -83,6 +83,11 @@ def _counters(device: torch.device, stream: int, capturing: bool) -> torch.Tenso
     return buf
 
 
+def _no_gradient(x: torch.Tensor, name: str, what: str) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: {name} asks for a gradient; this is a forward-only operator")
+
+
 def _pool_view(pool: torch.Tensor, layer: int, what: str):
     """AkvPagedPool of one layer, and the pool's heads, head_dim and type."""
     shape = pool.shape
@@ -93,6 +98,7 @@ def _pool_view(pool: torch.Tensor, layer: int, what: str):
     dtype = _DTYPES.get(torch_dtype)
     if dtype is None:
         raise ValueError(f"{what}: pool dtype must be float16, bfloat16 or float32, got {torch_dtype}")
+    _no_gradient(pool, "pool", what)
     n, layers, _, heads, bs, dim = shape
     return _POOL(pool.data_ptr(), n, layers, heads, bs, dim, dtype, layer, 0), heads, dim, torch_dtype
 
@@ -128,8 +134,7 @@ def _heads_view(x: torch.Tensor, dim: int, dtype: torch.dtype, device: torch.dev
     token, head, step = x.stride()
     if step != 1 and dim > 1:
         raise ValueError(f"{what}: {name}'s head_dim must be contiguous")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: {name} asks for a gradient; this is a forward-only operator")
+    _no_gradient(x, name, what)
     return _HEADS(x.data_ptr(), token, head)
 
 
@@ -189,6 +194,7 @@ def _check_bounds(bounds: torch.Tensor, pool: torch.Tensor, what: str) -> None:
             or not bounds.is_contiguous():
         raise ValueError(f"{what}: bounds must be a contiguous {(n, L, H, 2, D)} {pool.dtype} tensor on {pool.device}, "
                          f"got {tuple(bounds.shape)} {bounds.dtype} on {bounds.device}")
+    _no_gradient(bounds, "bounds", what)
 
 
 @lru_cache(maxsize=1024)
@@ -280,6 +286,18 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
             oview = _heads_view(query_out, dim, dtype, dev, "query_out", what)
     elif query_out is not None:
         raise ValueError(f"{what}: query_out without query")
+    rptr, positions, rotary = None, 0, 0
+    if rope is not None:
+        if rope.dim() != 2 or rope.dtype != torch.float32 or rope.device != dev or not rope.is_contiguous():
+            raise ValueError(f"{what}: rope must be a contiguous float32 [positions, rotary_dim] tensor on {dev}")
+        _no_gradient(rope, "rope", what)
+        if rope.data_ptr() % 16:
+            raise ValueError(f"{what}: rope must start on a 16-byte boundary")
+        rptr, (positions, rotary) = rope.data_ptr(), rope.shape
+    bptr = None
+    if bounds is not None:
+        _check_bounds(bounds, pool, what)
+        bptr = bounds.data_ptr()
     if not pool.is_cuda and not _require_cuda(pool, what):
         return query_out
     b, rows, _, tables, lengths = _batch_view(tables, lengths, dev, what)
@@ -291,17 +309,6 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
         if starts.shape != (rows + 1,):
             raise ValueError(f"{what}: starts must be [{rows + 1}], got {tuple(starts.shape)}")
         sptr = starts.data_ptr()
-    rptr, positions, rotary = None, 0, 0
-    if rope is not None:
-        if rope.dim() != 2 or rope.dtype != torch.float32 or rope.device != dev or not rope.is_contiguous():
-            raise ValueError(f"{what}: rope must be a contiguous float32 [positions, rotary_dim] tensor on {dev}")
-        if rope.data_ptr() % 16:
-            raise ValueError(f"{what}: rope must start on a 16-byte boundary")
-        rptr, (positions, rotary) = rope.data_ptr(), rope.shape
-    bptr = None
-    if bounds is not None:
-        _check_bounds(bounds, pool, what)
-        bptr = bounds.data_ptr()
 
     def call() -> None:
         st = _status(dev, status, _capturing())
@@ -366,6 +373,7 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, layer: int, tables,
     dtype = _DTYPES.get(bounds.dtype)
     if dtype is None:
         raise ValueError(f"{what}: bounds dtype must be float16, bfloat16 or float32, got {bounds.dtype}")
+    _no_gradient(bounds, "bounds", what)
     keep, first, last = int(keep), int(first), int(last)
     if keep < 1 or first < 0 or last < 0 or first + last > keep:
         raise ValueError(f"{what}: needs keep >= 1 and 0 <= first + last <= keep, got {keep}, {first}, {last}")

@@ -76,3 +76,28 @@ def test_the_work_space_is_enough_for_every_alignment(dtype):
                 rc = N.lib.akv_paged_attention(A._POOL(1 << 20, *geometry), batch, heads, group, 1.0, 0,
                                                1 << 20 if keep else None, keep, heads, None, 1 << 20, need, None, None, None)
                 assert rc == N.AKV_ERR_INVALID_ARG and "counters" in N.last_error(), (dim, group, at, N.last_error())
+
+
+def _meta(*shape, dtype=torch.bfloat16, **kw):
+    return torch.empty(shape, dtype=dtype, device="meta", **kw)
+
+
+def test_every_input_that_asks_for_a_gradient_is_refused():
+    pool, asks = _meta(8, 2, 2, 2, 16, 64), _meta(8, 2, 2, 2, 16, 64, requires_grad=True)
+    bounds, asks_b = _meta(8, 2, 2, 2, 64), _meta(8, 2, 2, 2, 64, requires_grad=True)
+    q, k = _meta(3, 4, 64), _meta(3, 2, 64)
+    calls = [
+        ("pool", lambda: A.paged_attention(q, asks, 0, None, None)),
+        ("pool", lambda: A.kv_append(asks, 0, k, k, None, None)),
+        ("pool", lambda: A.key_bounds(asks, 0, None, None)),
+        ("bounds", lambda: A.key_bounds(pool, 0, None, None, asks_b)),
+        ("bounds", lambda: A.kv_append(pool, 0, k, k, None, None, bounds=asks_b)),
+        ("bounds", lambda: A.select_blocks(q, asks_b, 0, None, None, 5, block_size=16)),
+        ("rope", lambda: A.kv_append(pool, 0, k, k, None, None, rope=_meta(9, 64, dtype=torch.float32, requires_grad=True))),
+    ]
+    for name, call in calls:
+        with pytest.raises(ValueError, match=f"{name} asks for a gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    A.select_blocks(q, bounds, 0, None, None, 5, block_size=16)
