@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_append(AppendParams p) {
 #pragma unroll 4
         for (int32_t r = q; r < in0; r += 4) {
           float x[kV], y[kV] = {};
-          load_word<T, kV>(x, tile + r * p.kv.row_bytes, ln.a);
-          if (ln.b >= 0) load_word<T, kV>(y, tile + r * p.kv.row_bytes, ln.b);
+          load_word<T, kV>(x, tile + static_cast<int64_t>(r) * p.kv.row_bytes, ln.a);
+          if (ln.b >= 0) load_word<T, kV>(y, tile + static_cast<int64_t>(r) * p.kv.row_bytes, ln.b);
           take(x, y);
         }
 #pragma unroll 4

@@ -368,3 +368,31 @@ def test_what_attend_reports_is_the_batch_s_own():
     batch.advance([[1], [2]])  # the tables are made anew
     batch.append(0, x, x)
     assert torch.equal(batch.attend(0, x, check=True), x)
+
+
+# ── one block of more than 2^31 bytes per head ───────────────────────────────
+def test_rows_beyond_32_bits_inside_a_block():
+    """The earlier keys of a first block are read for its bounds, and a row is
+    attended over, where a position's bytes start beyond 2^31 in its head's tile."""
+    bs, D, n = 1 << 22, 256, 2_200_001
+    pool = torch.zeros((1, 1, 2, 1, bs, D), device=DEV)  # 8.6 GB
+    far = 2_150_000
+    assert far * D * 4 > 2 ** 31
+    g = _gen(1)
+    kfar, vfar, k, v = (_randn(g, D, dtype=F32) for _ in range(4))
+    pool[0, 0, 0, 0, far], pool[0, 0, 1, 0, far] = kfar, vfar
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([n], dtype=torch.int32, device=DEV)
+    bounds = torch.full((1, 1, 1, 2, D), 7.0, device=DEV)
+    A.kv_append(pool, 0, k.view(1, 1, D), v.view(1, 1, D), table, lengths, bounds=bounds, check=True)
+    assert torch.equal(pool[0, 0, 0, 0, n - 1], k) and torch.equal(pool[0, 0, 1, 0, n - 1], v)
+    three = torch.stack([kfar, k, torch.zeros_like(k)])
+    assert torch.equal(bounds[0, 0, 0, 0], three.amin(0)) and torch.equal(bounds[0, 0, 0, 1], three.amax(0))
+    q = torch.zeros(1, 1, D, device=DEV)
+    q[0, 0] = 30 * kfar / (kfar @ kfar)
+    out = A.paged_attention(q, pool, 0, table, lengths, scale=1.0, check=True)
+    x = torch.stack([q[0, 0].double() @ kfar.double(), q[0, 0].double() @ k.double()])
+    w = torch.exp(x - 30)
+    want = (w[0] * vfar.double() + w[1] * v.double()) / (w.sum() + (n - 2) * math.exp(-30))
+    # scores of 30 in 32 bits, to base 2 and taken off one another: 3 * 2^-24 * 43 of a weight, with exp2's 2^-21
+    assert ((out[0, 0].double() - want).abs() <= 2e-5 * (vfar.double().abs() + 1e-6)).all()
