@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads) k_bounds(AppendParams p) {
     const int32_t s = static_cast<int32_t>(it / per_row);
     const int32_t block = static_cast<int32_t>(it % per_row / p.kv.heads), h = static_cast<int32_t>(it % p.kv.heads);
     const int32_t len = akv_held(p.tab, bl, s);
-    if (block == 0 && h == 0 && lane == 0 && p.tab.lengths[s] > len)
+    if (block == 0 && h == 0 && lane == 0 && p.tab.lengths[s] != len)
       akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, p.tab.lengths[s], p.tab.width);
     const int64_t from = static_cast<int64_t>(block) << bl;
     if (from >= len) continue;

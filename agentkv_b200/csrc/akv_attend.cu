@@ -719,10 +719,10 @@ __global__ void __launch_bounds__(kThreads, Eng::kCtas) k_attend(AttendParams p)
       search.find(sh, x, units, s, rest);
     }
   }
-  // rows that hold nothing, and lengths that the table cannot hold
+  // rows that hold nothing, and lengths that no table can hold
   for (int32_t r = blockIdx.x; r < p.tab.rows; r += gridDim.x) {
     const int32_t n = akv_held(p.tab, p.kv.bs_log2, r);
-    if (threadIdx.x == 0 && p.tab.lengths[r] > n)
+    if (threadIdx.x == 0 && p.tab.lengths[r] != n)
       akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, r, p.tab.lengths[r], p.tab.width);
     if (n == 0) {
       const int32_t heads = p.kv.heads * p.group;

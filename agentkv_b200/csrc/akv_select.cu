@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kSelectThreads) k_select(SelectParams p) {
   const int32_t s = blockIdx.x / p.kv.heads, h = blockIdx.x % p.kv.heads;
   const int32_t n = blocks_of(p, s);
   int32_t* out = p.selected + static_cast<int64_t>(blockIdx.x) * p.keep;
-  if (tid == 0 && h == 0 && p.tab.lengths[s] > akv_held(p.tab, p.kv.bs_log2, s))
+  if (tid == 0 && h == 0 && p.tab.lengths[s] != akv_held(p.tab, p.kv.bs_log2, s))
     akv_fail(p.st, AKV_ERR_OUT_OF_RANGE, s, p.tab.lengths[s], p.tab.width);
   if (n <= p.keep) {
     for (int32_t i = tid; i < p.keep; i += kSelectThreads) out[i] = i < n ? i : -1;

@@ -659,7 +659,9 @@ AKV_API int akv_alloc_replay(const AkvAllocState* st, const int32_t* log, int64_
  * sequences: row s holds lengths[s] tokens (0: a padding row), token t of it
  * in block tables[s * table_stride + t / block_size], position
  * t % block_size.  tables and lengths are DEVICE arrays; table entries behind
- * a row's last block are not read.  Strides are in elements. */
+ * a row's last block are not read.  A length below 0, or above table_width *
+ * block_size, is reported (AKV_ERR_OUT_OF_RANGE); what reads the pages takes
+ * it as 0 or as that many.  Strides are in elements. */
 enum { AKV_F32 = 0, AKV_F16 = 1, AKV_BF16 = 2 };
 
 typedef struct AkvPagedPool {

@@ -396,3 +396,32 @@ def test_rows_beyond_32_bits_inside_a_block():
     want = (w[0] * vfar.double() + w[1] * v.double()) / (w.sum() + (n - 2) * math.exp(-30))
     # scores of 30 in 32 bits, to base 2 and taken off one another: 3 * 2^-24 * 43 of a weight, with exp2's 2^-21
     assert ((out[0, 0].double() - want).abs() <= 2e-5 * (vfar.double().abs() + 1e-6)).all()
+
+
+# ── lengths that are no lengths ──────────────────────────────────────────────
+@pytest.mark.parametrize("wrong", [-1, -2 ** 31, 3 * 16 + 1, 2 ** 31 - 1])
+def test_lengths_that_no_row_can_have_are_reported_by_every_operator(wrong):
+    """And taken as 0, or as what the table holds, by those that read."""
+    g = _gen(8)
+    pool = _randn(g, 6, 1, 2, 2, 16, 64, dtype=BF16)
+    table = torch.arange(6, dtype=torch.int32, device=DEV).view(2, 3)
+    right = torch.tensor([20, 0 if wrong < 0 else 48], dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([20, wrong], dtype=torch.int32, device=DEV)
+    q = _randn(g, 2, 8, 64, dtype=BF16)
+    bounds = A.key_bounds(pool, 0, table, right, check=True)
+    sel = A.select_blocks(q, bounds, 0, table, right, 2, block_size=16, check=True)
+    out = A.paged_attention(q, pool, 0, table, right, check=True)
+    st = torch.zeros(8, dtype=torch.int32, device=DEV)
+
+    def reported(row=1):
+        code, index, bid = K.read_status(st)[:3]
+        st.zero_()
+        return (code, index, bid) == (N.AKV_ERR_OUT_OF_RANGE, row, wrong)
+
+    assert torch.equal(A.paged_attention(q, pool, 0, table, lengths, status=st), out) and reported()
+    assert torch.equal(A.select_blocks(q, bounds, 0, table, lengths, 2, block_size=16, status=st), sel) and reported()
+    assert torch.equal(A.key_bounds(pool, 0, table, lengths, status=st), bounds) and reported()
+    before = pool.clone()
+    A.kv_append(pool, 0, q[:, :2], q[:, 2:4], table, lengths, status=st)
+    assert K.read_status(st)[:2] == (N.AKV_ERR_OUT_OF_RANGE, 1)
+    assert torch.equal(pool[table[1].long()], before[table[1].long()])
