@@ -24,7 +24,8 @@ wait; its work space comes from PyTorch's allocator for that stream, so calls
 on several streams and captured calls do not share any.  Ids and lengths that
 only the device can check are reported in ``status`` (an AkvStatus record, by
 default one per device and stream, and one per device for captured calls;
-``check=True`` waits and raises BlockOpError, which clears it).  The tokens
+``check=True`` waits and raises BlockOpError, which clears it, and is refused
+while capturing).  The tokens
 concerned are left out; while the record holds an error, kv_append and
 key_bounds write nothing, as the framework's other writes (the reads go on).
 That starts with the call that reports it, so any of such a call's other tokens
@@ -55,10 +56,13 @@ _capturing = torch._C._cuda_isCurrentStreamCapturing
 _current_device = torch._C._cuda_getDevice
 
 
-def _status(device: torch.device, status: Optional[torch.Tensor], capturing: bool) -> Optional[torch.Tensor]:
+def _status(device: torch.device, status: Optional[torch.Tensor], capturing: bool,
+            check: bool = False) -> Optional[torch.Tensor]:
     """The caller's status record or the default one.  A captured call uses a
     record of the device that an eager call made (a record made while capturing
     would be cleared by replays of that one graph only); before any, none."""
+    if check and capturing:
+        raise RuntimeError("check=True waits for the call: not while capturing")
     if status is not None:
         if status.dtype != torch.int32 or status.device != device or status.numel() * 4 < N.STATUS_BYTES:
             raise ValueError("status must be an int32 tensor of 8 elements on the pool's device")
@@ -311,7 +315,7 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
         sptr = starts.data_ptr()
 
     def call() -> None:
-        st = _status(dev, status, _capturing())
+        st = _status(dev, status, _capturing(), check)
         rc = N.lib.akv_kv_append(p, b, kview, vview, tokens, sptr, rptr, positions, rotary, interleaved, qview, oview,
                                  heads, bptr, None if st is None else st.data_ptr(), stream_handle(dev))
         if rc:
@@ -344,7 +348,7 @@ def key_bounds(pool: torch.Tensor, layer: int, tables, lengths, bounds: Optional
     b, _, _, tables, lengths = _batch_view(tables, lengths, dev, what)
 
     def call() -> None:
-        st = _status(dev, status, _capturing())
+        st = _status(dev, status, _capturing(), check)
         N.check(N.lib.akv_key_bounds(p, b, bounds.data_ptr(), None if st is None else st.data_ptr(),
                                      stream_handle(dev)))
         if check and st is not None:
@@ -390,7 +394,7 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, layer: int, tables,
         raise ValueError(f"{what}: {rows} queries for {batch} rows")
 
     def call() -> None:
-        st = _status(dev, status, _capturing())
+        st = _status(dev, status, _capturing(), check)
         scratch = query.new_empty(max(0, N.lib.akv_select_blocks_scratch_bytes(rows, H, width, keep)),
                                   dtype=torch.uint8)
         rc = N.lib.akv_select_blocks(p, bounds.data_ptr(), b, qview, group, keep, first, last, selected.data_ptr(),
@@ -455,7 +459,7 @@ def paged_attention(query: torch.Tensor, pool: torch.Tensor, layer: int, tables,
 
     def call() -> None:
         capturing = _capturing()
-        st, stream = _status(dev, status, capturing), stream_handle(dev)
+        st, stream = _status(dev, status, capturing, check), stream_handle(dev)
         scratch = query.new_empty(_attention_scratch(p[8:], rows, width, group, keep), dtype=torch.uint8)
         rc = N.lib.akv_paged_attention(
             p, b, qview, group, dim ** -0.5 if scale is None else scale, min(window, (1 << 31) - 1), sel, keep, oview,

@@ -425,3 +425,30 @@ def test_lengths_that_no_row_can_have_are_reported_by_every_operator(wrong):
     A.kv_append(pool, 0, q[:, :2], q[:, 2:4], table, lengths, status=st)
     assert K.read_status(st)[:2] == (N.AKV_ERR_OUT_OF_RANGE, 1)
     assert torch.equal(pool[table[1].long()], before[table[1].long()])
+
+
+def test_a_captured_call_refuses_to_wait():
+    """check=True while capturing: refused before anything is recorded, so that
+    the capture goes on."""
+    g = _gen(2)
+    pool = _randn(g, 4, 1, 2, 2, 16, 64, dtype=BF16)
+    table = torch.arange(4, dtype=torch.int32, device=DEV).view(2, 2)
+    lengths = torch.tensor([20, 5], dtype=torch.int32, device=DEV)
+    q = _randn(g, 2, 8, 64, dtype=BF16)
+    bounds = A.key_bounds(pool, 0, table, lengths, check=True)
+    want = A.paged_attention(q, pool, 0, table, lengths, check=True)
+
+    def calls():
+        for call in (lambda: A.paged_attention(q, pool, 0, table, lengths, check=True),
+                     lambda: A.select_blocks(q, bounds, 0, table, lengths, 1, first=0, last=0, block_size=16, check=True),
+                     lambda: A.key_bounds(pool, 0, table, lengths, bounds, check=True),
+                     lambda: A.kv_append(pool, 0, q[:, :2], q[:, 2:4], table, lengths, check=True)):
+            with pytest.raises(RuntimeError, match="capturing"):
+                call()
+        return A.paged_attention(q, pool, 0, table, lengths)
+
+    graph, out = _capture(calls)
+    before = pool.clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(pool, before)
