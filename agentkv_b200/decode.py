@@ -60,6 +60,7 @@ class DecodeBatch:
         data = pool._allocator._kv_data
         self._data = data
         ids = [pool.get_block_ids(h) for h in self.handles]
+        self._all_held([len(b) for b in ids])
         need = max([len(b) for b in ids], default=0)
         self.width = max(1, need) if width is None else int(width)
         self.tables = torch.zeros((self.rows, self.width), dtype=torch.int32, device=data.device)
@@ -81,6 +82,14 @@ class DecodeBatch:
             else:
                 A._check_bounds(bounds, data, "DecodeBatch")
                 self.bounds = bounds
+
+    def _all_held(self, blocks: Sequence[int]) -> None:
+        """Refuses an agent whose tokens are more than its blocks hold (a root
+        made of a prompt that is not in the pool yet)."""
+        bs = self.pool.block_size
+        for h, n in zip(self.handles, blocks):
+            if len(h.tokens) > n * bs:
+                raise ValueError(f"DecodeBatch: an agent has {len(h.tokens)} tokens in {n} blocks of {bs}")
 
     def _upload(self, ids: List[List[int]]) -> None:
         need = max([len(b) for b in ids], default=0)
@@ -118,6 +127,7 @@ class DecodeBatch:
             self.check()
         counts = [len(t) for t in tokens]
         held = [len(pool.get_block_ids(h)) for h in self.handles]  # refuses a freed agent before anything changes
+        self._all_held(held)
         if self._fixed:
             for h, n in zip(self.handles, counts):
                 if len(h.tokens) + n > self.width * bs:

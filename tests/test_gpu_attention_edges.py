@@ -452,3 +452,94 @@ def test_a_captured_call_refuses_to_wait():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(pool, before)
+
+
+# ── DecodeBatch over the shared tree ─────────────────────────────────────────
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_agents_on_a_matched_prefix_decode_together(dtype):
+    """One agent commits its prompt's whole blocks; others match them (in whole,
+    in part, by create_root), bring their own rest and go on, forks among them: outputs and
+    bytes against a model that keeps each agent's keys and values apart."""
+    H, G, D, L, bs = 2, 2, 64, 2, 8
+    t = {"bfloat16": BF16, "float32": F32}[dtype]
+    u = torch.finfo(t).eps / 2
+    pool = AgentKVPool(config=PoolConfig(total_blocks=200, block_size=bs, num_layers=L, num_kv_heads=H, head_dim=D,
+                                         dtype=dtype, device="cuda"))
+    g = _gen(31)
+    model = {}  # handle id -> [[keys, values] of each layer]
+
+    def step(batch, new, **kw):
+        batch.advance(new)
+        counts = [len(n) for n in new]
+        for layer in range(L):
+            k, v = (_randn(g, sum(counts), H, D, dtype=t) for _ in range(2))
+            batch.append(layer, k, v)
+            at = 0
+            for h, n in zip(batch.handles, counts):
+                old = model[h.handle_id][layer]
+                model[h.handle_id][layer] = [torch.cat([old[0], k[at:at + n]]), torch.cat([old[1], v[at:at + n]])]
+                at += n
+            q = _randn(g, batch.rows, H * G, D, dtype=t)
+            out = batch.attend(layer, q, **kw)
+            batch.check()
+            data = pool._allocator._kv_data
+            for i, h in enumerate(batch.handles):
+                keys, values = model[h.handle_id][layer]
+                ids = torch.tensor(pool.get_block_ids(h), device=DEV)
+                held = data[ids, layer].permute(1, 2, 0, 3, 4).reshape(2, H, -1, D)[:, :, :len(h.tokens)]
+                assert torch.equal(held[0].transpose(0, 1), keys) and torch.equal(held[1].transpose(0, 1), values)
+                x = torch.einsum("hgd,nhd->hgn", q[i].view(H, G, D).double(), keys.double()) * D ** -0.5
+                want = torch.einsum("hgn,nhd->hgd", torch.softmax(x, 2), values.double()).reshape(H * G, D)
+                assert ((out[i].double() - want).abs() <= u * want.abs() + 3e-5 * 6).all()
+
+    def empty(h):
+        model[h.handle_id] = [[torch.zeros(0, H, D, dtype=t, device=DEV)] * 2 for _ in range(L)]
+        return h
+
+    def follow(h, of, n):
+        model[h.handle_id] = [[x[:n] for x in layer] for layer in model[of.handle_id]]
+        return h
+
+    prompt = list(range(100, 137))  # 37 tokens: 4 blocks of 8 and 5 more
+    a = empty(pool.create_root([]))
+    first = pool.decode_batch([a], bounds=True)
+    step(first, [prompt])
+    pool.commit_prefix(a, 32)
+    step(first, [[7]])                              # its own last block, behind the shared ones
+    b, n = pool._tree.match_prefix(prompt + [1, 2])  # all that was committed
+    assert n == 32
+    follow(b, a, 32)
+    c = pool.create_root(prompt[:32])                # the same, to the token
+    follow(c, a, 32)
+    d, n = pool._tree.match_prefix(prompt[:32] + [9] * 20)
+    follow(d, a, 32)
+    batch = pool.decode_batch([b, c, d, a], rows=5, bounds=first.bounds)
+    step(batch, [prompt[32:] + [1, 2], [], [9] * 20, [8]])
+    step(batch, [[3], [4], [5], [6]], keep=7)         # no row has more than 7 blocks: all of them
+    pool.commit_prefix(d, 16)                         # deeper in the tree
+    e, n = pool._tree.match_prefix(prompt[:32] + [9] * 20)
+    assert n == 48
+    follow(e, d, 48)
+    f = pool.fork(e)
+    follow(f, e, 48)
+    for h in (b, c):
+        pool.free(h)
+    last = pool.decode_batch([d, e, f, a])
+    for _ in range(bs + 1):
+        step(last, [[1], [2], [3], [4]])
+    pool._allocator.check()
+
+
+def test_tokens_without_blocks_are_refused():
+    """A root made of a prompt holds its tokens, but no key or value of those
+    that no prefix matched."""
+    pool, _, _ = _batch()
+    h = pool.create_root(list(range(9)))
+    with pytest.raises(ValueError, match="9 tokens in 0 blocks"):
+        pool.decode_batch([h])
+    pool.allocate_blocks(h, 3)  # for keys and values that come by other means
+    batch = pool.decode_batch([h])
+    pool.append_tokens(h, [1] * 4)
+    with pytest.raises(ValueError, match="13 tokens in 3 blocks"):
+        batch.advance([[1]])
+    assert len(h.tokens) == 13 and len(pool.get_block_ids(h)) == 3
