@@ -46,18 +46,6 @@ struct AppendParams {
   AkvStatus* st;
 };
 
-// min / max that a NaN on either side makes NaN
-AKV_DEV float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-AKV_DEV float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // New tokens of row s, and how many blocks they fall into.
 AKV_DEV int32_t new_tokens(const AppendParams& p, int32_t s) {
   if (p.starts == nullptr) return p.tab.lengths[s] > 0 ? 1 : 0;

@@ -91,6 +91,18 @@ AKV_DEV AkvPack<T, N> akv_pack(float (&x)[N]) {
   return w;
 }
 
+// min / max that a NaN on either side makes NaN
+AKV_DEV float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+AKV_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Waits until the launches before this one in the stream have ended and their
 // writes can be seen; a launch without the programmatic attribute passes.
 AKV_DEV void akv_grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
