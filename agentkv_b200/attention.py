@@ -257,7 +257,8 @@ def kv_append(pool: torch.Tensor, layer: int, key: torch.Tensor, value: torch.Te
     first rotary_dim dimensions of each new key by its position, pairs
     (i, i + rotary_dim / 2), or neighbours with ``interleaved``.  ``query``
     ([tokens, query heads, head_dim]) is rotated the same way and returned
-    (in ``query_out`` when given, which may be query itself).  ``bounds``
+    (in ``query_out`` when given, which may be query itself; rows of padding are
+    left as they are there, and undefined without it).  ``bounds``
     ([blocks, layers, heads, 2, head_dim], see key_bounds) is brought up to
     date for the blocks written."""
     what = "kv_append"
@@ -334,7 +335,9 @@ def key_bounds(pool: torch.Tensor, layer: int, tables, lengths, bounds: Optional
     maximum, by dimension, of block b's keys (of a row's last block, those
     that the row holds).  Makes the [blocks, layers, heads, 2, head_dim]
     tensor (zeros elsewhere) when none is given.  kv_append keeps bounds up to date by
-    itself; this is for blocks that were written by other means."""
+    itself; this is for blocks that were written by other means.  Rows that
+    share a block hold equally many of its keys: of rows with one table and other
+    lengths (several new tokens of a sequence) give the longest alone."""
     what = "key_bounds"
     p = _pool_view(pool, layer, what)[0]
     n, L, _, H, _, D = pool.shape
@@ -369,7 +372,8 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, layer: int, tables,
     first and `last` last blocks and, of the others, those of the highest
     score: the sum, over the query heads that share the key head, of the
     highest score that a key within the block's ``bounds`` could have.  Of
-    equal scores the lower place is taken; a NaN score counts as the highest."""
+    equal scores the lower place is taken; a NaN score counts as the highest (an
+    infinite bound makes one where no query head of the group has the sign that meets it)."""
     what = "select_blocks"
     if bounds.dim() != 5 or bounds.shape[3] != 2 or not bounds.is_contiguous():
         raise ValueError(f"{what}: bounds must be a contiguous [blocks, layers, heads, 2, head_dim] tensor")
@@ -426,7 +430,10 @@ def paged_attention(query: torch.Tensor, pool: torch.Tensor, layer: int, tables,
     With ``return_lse`` also the float32 [rows, heads] natural
     logarithm of each softmax's sum (-inf for an empty row).  Several new
     tokens of one sequence are several rows with the same table and
-    their own lengths."""
+    their own lengths.  NaN and infinities in blocks that a row does not read, or behind
+    its last position, do not reach it; an infinite value among those that
+    take part makes its dimension infinite or NaN (a weight is held as a sum
+    of two 16-bit numbers, and infinity times either may be NaN)."""
     what = "paged_attention"
     p, kv_heads, dim, dtype = _pool_view(pool, layer, what)
     dev = pool.device

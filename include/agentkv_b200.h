@@ -726,7 +726,8 @@ AKV_API int akv_kv_append(const AkvPagedPool* pool, const AkvPageBatch* batch, c
                   void* stream);
 
 /* bounds (as above) of every block of every row, from the keys in the pool:
- * for blocks that were written by other means than akv_kv_append. */
+ * for blocks that were written by other means than akv_kv_append.  Rows that
+ * share a block hold equally many of its keys. */
 AKV_API int akv_key_bounds(const AkvPagedPool* pool, const AkvPageBatch* batch, void* bounds, AkvStatus* status,
                    void* stream);
 
@@ -738,7 +739,8 @@ AKV_API int akv_key_bounds(const AkvPagedPool* pool, const AkvPageBatch* batch, 
  * table (distinct, any order, the valid ones first and -1 behind them); only
  * their positions take part.  Scores are scaled by `scale`; sums, the
  * softmax's statistics and the output are held in 32 bits and the output is
- * rounded once.  A row in which nothing takes part gives 0 (lse -inf).  lse, when
+ * rounded once.  A row in which nothing takes part gives 0 (lse -inf).  An
+ * infinite value that takes part makes its dimension infinite or NaN.  lse, when
  * non-NULL, is float32 [rows][num_kv_heads * group]: the natural logarithm
  * of the sum of the scores' exponentials.
  *
@@ -762,7 +764,9 @@ AKV_API int akv_paged_attention(const AkvPagedPool* pool, const AkvPageBatch* ba
  * ceil(lengths[s] / block_size), with kmin, kmax the block's bounds (pool->data
  * is not read, bounds is as for akv_kv_append),
  *   score = sum over the group's query heads and d of max(q_d kmin_d, q_d kmax_d),
- * in 64 bits.  selected [rows][num_kv_heads][keep] gets ascending places in
+ * in 64 bits, as the sum over d of P_d kmax_d + N_d kmin_d with P_d and N_d the sums of
+ * the heads' positive and negative q_d (an infinite bound times a part that is 0 is
+ * NaN).  selected [rows][num_kv_heads][keep] gets ascending places in
  * the row's table, -1 behind them: all n where n <= keep; else the first
  * `first` and the last `last` blocks (first + last <= keep) and the
  * highest-scored of the others, the lowest place of equal ones.  A NaN score

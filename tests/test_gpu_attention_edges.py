@@ -543,3 +543,25 @@ def test_tokens_without_blocks_are_refused():
     with pytest.raises(ValueError, match="13 tokens in 3 blocks"):
         batch.advance([[1]])
     assert len(h.tokens) == 13 and len(pool.get_block_ids(h)) == 3
+
+
+# ── infinite values ──────────────────────────────────────────────────────────
+@pytest.mark.parametrize("dtype,D", [(F16, 64), (BF16, 128), (BF16, 80), (F32, 64), (BF16, 7)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_a_value_that_is_no_number_stays_in_its_dimension(dtype, D, value):
+    """Of its key head and row: infinite or NaN there, and all else as without it;
+    behind the row's last position it is not there at all."""
+    g = _gen(14)
+    pool = _randn(g, 12, 1, 2, 2, 16, D, dtype=dtype)
+    table = torch.arange(12, dtype=torch.int32, device=DEV).view(3, 4)
+    lengths = torch.tensor([50, 60, 7], dtype=torch.int32, device=DEV)
+    q = _randn(g, 3, 6, D, dtype=dtype)
+    clean, lse = A.paged_attention(q, pool, 0, table, lengths, return_lse=True, check=True)
+    pool[5, 0, 1, 1, 3, 2] = value   # row 1, position 19, key head 1, dimension 2
+    pool[8, 0, 1, 1, 7:, 2] = value  # row 2, behind its 7 tokens
+    pool[8, 0, 0, :, 7:] = value
+    pool[3, 0, :, :, 2:] = value     # row 0, behind its 50
+    out, l2 = A.paged_attention(q, pool, 0, table, lengths, return_lse=True, check=True)
+    assert not torch.isfinite(out[1, 3:, 2]).any()
+    out[1, 3:, 2] = clean[1, 3:, 2]
+    assert torch.equal(out, clean) and torch.equal(l2, lse)
