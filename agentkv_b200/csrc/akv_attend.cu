@@ -228,6 +228,8 @@ AKV_DEV uint32_t transpose8x8(uint32_t a) {
   return d;
 }
 
+// 2^x, off by 2^-22 of it at most, and 0 below 2^-126.  Both are far under half a step
+// of the 16-bit outputs (2^-8 of a value in bf16, 2^-11 in fp16); the 32-bit engine takes exp2f.
 AKV_DEV float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -238,7 +240,9 @@ AKV_DEV uint4 ld16(const char* p) { return __ldg(reinterpret_cast<const uint4*>(
 AKV_DEV uint2 ld8(const char* p) { return __ldg(reinterpret_cast<const uint2*>(p)); }
 
 // Compiled for kD = 64, 96, 128 and 256; the dimensions between (kExact false) take the
-// next one's products with zeros behind their own words.
+// next one's products with zeros behind their own words.  At 168 registers the form of
+// 128 spills 28 bytes a thread (68 for the dimensions between), that of 256 at 255
+// registers 16 (160); the others none.
 template <typename T, int kD, int kN, bool kExact>
 struct MmaEngine {
   using Type = T;

@@ -19,7 +19,8 @@
 //
 // What bounds it: 2 head_dim elements read per block and key head.  Measured: bounds
 // of 32 rows' 41,700 blocks (171 MB, 8 key heads of 128) scored in 62 us, 2.8 TB/s
-// (what issues is each score's sum over the lanes), chosen from in 22 us.
+// (what issues is each score's sum over the lanes; about 100 bytes a thread are
+// spilled at 128 registers), chosen from in 22 us.
 #include <climits>
 
 #include "akv_paged.cuh"
