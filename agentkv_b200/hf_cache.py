@@ -100,7 +100,7 @@ class AgentKVCache(DynamicCache):
         reads them where they lie, with attend() (called after store(), for
         each layer).  Not while capturing: a replay would write this step's
         places, whose blocks may have become another agent's."""
-        if A._capturing():
+        if key_states.is_cuda and A._capturing():
             raise RuntimeError("AgentKVCache.store: not while capturing (DecodeBatch.append can be captured)")
         self._write(key_states, value_states, layer_idx)
         self._layer_done(layer_idx)

@@ -5,6 +5,7 @@ calls whose inputs move on."""
 import math
 import subprocess
 import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -297,7 +298,8 @@ print("right")
 def test_first_launches_of_every_form_inside_a_capture():
     """A pool's making loads the kernels: head dims and alignments of every
     form can be captured without an eager call of theirs before."""
-    r = subprocess.run([sys.executable, "-c", _FIRST], capture_output=True, text=True, timeout=300)
+    r = subprocess.run([sys.executable, "-c", _FIRST], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parents[1])
     assert r.returncode == 0 and "right" in r.stdout, r.stderr[-2000:]
 
 
